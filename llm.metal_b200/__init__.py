@@ -21,6 +21,7 @@ c_u32_p = C.POINTER(C.c_uint32)
 
 B200_MAX_PEERS = 8
 B200_WT_Q8, B200_WT_F16, B200_WT_BF16, B200_WT_F32 = 0, 1, 2, 3
+B200_PAGED_MAX_REQ, B200_PAGED_NO_PAGES, B200_PAGED_BAD_LENGTH, B200_PAGED_BAD_PAGE = 1024, 1, 2, 4
 B200_IN_VEC, B200_IN_RESID, B200_IN_EMBED, B200_IN_POSTNORM = 0, 1, 2, 3
 B200_OUT_STORE, B200_OUT_GLU, B200_OUT_GATED, B200_OUT_STREAMS = 0, 1, 2, 3
 B200_ACT_SILU, B200_ACT_GELU_TANH, B200_ACT_RELU2 = 0, 1, 2
@@ -227,6 +228,29 @@ class RowsPostnormArgs(C.Structure):
                 ("coef", C.c_void_p), ("out", C.c_void_p), ("out_h", C.c_void_p)]
 
 
+class PagesArgs(C.Structure):
+    """b200_pages_args (include/llmb200_paged_kernels.h)."""
+    _fields_ = [(n, C.c_int) for n in ("n_req", "page", "table_ld", "n_pages", "max_rows")] + \
+               [(n, C.c_void_p) for n in ("d_len", "d_len_out", "d_new", "d_base", "d_table", "d_free", "d_free_n", "d_free_n_out", "d_row_start",
+                                          "d_slot", "d_pos", "d_status")] + [("use_pdl", C.c_int)]
+
+
+class PagedStoreArgs(C.Structure):
+    """b200_paged_store_args (include/llmb200_paged_kernels.h)."""
+    _fields_ = [(n, C.c_int) for n in ("wtype", "n_q", "n_kv", "hd", "page", "n_pages", "max_rows")] + [("eps", C.c_float), ("d_qkv", C.c_void_p), ("qkv_ld", C.c_longlong)] + \
+               [(n, C.c_void_p) for n in ("d_q_gamma", "d_k_gamma", "d_inv_freq", "d_rows", "d_slot", "d_pos", "d_k_pool", "d_v_pool", "d_q")] + \
+               [("q_ld", C.c_longlong), ("d_status", C.c_void_p), ("use_pdl", C.c_int)]
+
+
+class PagedAttnArgs(C.Structure):
+    """b200_paged_attn_args (include/llmb200_paged_kernels.h)."""
+    _fields_ = [(n, C.c_int) for n in ("wtype", "n_q", "n_kv", "hd", "page", "n_pages", "max_rows")] + [("scale", C.c_float), ("d_q", C.c_void_p), ("q_ld", C.c_longlong)] + \
+               [("d_k_pool", C.c_void_p), ("d_v_pool", C.c_void_p), ("d_out", C.c_void_p), ("out_ld", C.c_longlong), ("n_req", C.c_int)] + \
+               [("d_row_start", C.c_void_p), ("d_len", C.c_void_p), ("d_table", C.c_void_p), ("table_ld", C.c_int), ("n_groups", C.c_int)] + \
+               [("d_group_start", C.c_void_p), ("d_prefix_len", C.c_void_p), ("d_prefix_table", C.c_void_p), ("prefix_ld", C.c_int)] + \
+               [("d_work", C.c_void_p), ("work_bytes", C.c_size_t), ("d_status", C.c_void_p), ("use_pdl", C.c_int)]
+
+
 class WMat(C.Structure):
     _fields_ = [("mbuf", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int), ("nb", C.c_int)]
 
@@ -281,6 +305,7 @@ SYMBOLS_MAIN = {
                                 "b200_rms_norm_rows_h", "b200_rms_norm_bwd_rows_h", "b200_attn_train_fwd_h", "b200_attn_train_fwd_tc", "b200_attn_train_bwd_tc",
                                 "b200_silu_mul_rows_h", "b200_silu_mul_bwd_rows_h", "b200_softmax_ce_rows_h",
                                 "b200_grpo_policy_grad", "b200_scale", "b200_sgd_apply_f16", "b200_gelu_mul_rows", "b200_gelu_mul_bwd_rows", "b200_add"],
+    "llmb200_paged_kernels.h": ["b200_pages_extend", "b200_pages_release", "b200_paged_store", "b200_paged_attn_work_bytes", "b200_paged_attn"],
     "llmb200_sft.h": ["sft_state_create", "sft_state_free", "sft_train_step", "forward_to_logits", "sft_backward",
                       "sft_get_logits", "sft_get_dlogits", "sft_get_x_cpu", "sft_get_losses_cpu", "sft_get_seq_len",
                       "sft_get_vocab_size", "sft_get_d_model", "sft_get_lora_rank", "sft_get_n_layers",
@@ -424,6 +449,10 @@ def lib():
         "b200_sgd_apply_f16": (i, [vp, vp, sz, fl, vp]),
         "b200_gelu_mul_rows": (i, [vp, i, i, vp, vp]), "b200_gelu_mul_bwd_rows": (i, [vp, vp, i, i, vp, vp]),
         "b200_add": (i, [vp, vp, vp, sz, vp]),
+        # ---- llmb200_paged_kernels.h
+        "b200_pages_extend": (i, [C.POINTER(PagesArgs), vp]), "b200_pages_release": (i, [C.POINTER(PagesArgs), vp]),
+        "b200_paged_store": (i, [C.POINTER(PagedStoreArgs), vp]),
+        "b200_paged_attn_work_bytes": (sz, [C.POINTER(PagedAttnArgs)]), "b200_paged_attn": (i, [C.POINTER(PagedAttnArgs), vp]),
         # ---- llmb200_sft.h
         "sft_state_create": (vp, [vp, i, i, fl]), "sft_state_free": (None, [vp]),
         "sft_train_step": (fl, [vp, c_u32_p, c_u32_p, fl]),

@@ -1,0 +1,445 @@
+// Attention of a step's new rows over pages (sm_100a): each row over its request's own tokens, and over a prefix that its group shares
+// (paged_plan.cuh: how the work is cut).
+//
+// attn_few_kernel: a warp to itself, 16 query rows against a stretch of keys on mma.sync, m16n8k16, 16 keys a unit. Keys and values come with cp.async
+// into a ring of the warp's own, two units ahead; scores, weights and sums stay in registers, one pass with a running maximum. What bounds it
+// is memory: 16 rows take 64 operations a byte of cache at most, and the few warps of an SM hold enough bytes in flight. Warps share nothing, so that there is
+// no barrier in the loop. Scores, maxima, sums and results are fp32; weights are rounded to the cache's type for the second product, by at most
+// half a step each, which is what the results' own rounding is.
+// attn_join_kernel: a warp to each (row, query head) whose keys were cut, over the pieces in the order of the line.
+#include "paged_plan.cuh"
+
+#include <cuda_bf16.h>
+
+#include <limits.h>
+#include <type_traits>
+
+extern unsigned long long g_b200_launches;
+
+namespace {
+
+constexpr int FEW_ROWS = 16, FEW_KEYS = 16, FEW_WARPS = 4, FEW_STAGES = 3, FEW_LEAST = 4;
+constexpr int JOIN_WARPS = 8;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ float ex2(float x)                // 2^x, 2 ulp, 0 for -inf
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <typename T> __device__ __forceinline__ float to_float(uint16_t b)
+{
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(b));
+    else return __uint_as_float((uint32_t)b << 16);
+}
+// Whether one of the eight elements of a 16-byte word is infinite or NaN.
+template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v)
+{
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
+    return any;
+}
+
+// Where a kernel's pieces lie in d_work: [slot][rt][hd] sums and [slot][rt] (largest score, sum). A tile's piece of worker w is in slot tile + w: the
+// number of a piece never falls from one to the next on the line and one of the two grows.
+struct Pieces { float *acc; float2 *top; long long workers; };
+
+// Units of a worker: equal stretches, and none so short that joining costs more than it spreads.
+__device__ __forceinline__ long long stretch(long long units, long long workers, int least)
+{
+    const long long per = (units + workers - 1) / workers;
+    return per < least ? least : per;
+}
+
+// Whether the rows of a request have keys in a prefix.
+__device__ __forceinline__ int group_of(const Plan &p, int r)
+{
+    if (!p.n_groups || r < p.group[0] || r >= p.group[p.n_groups]) return -1;
+    const int g = last_at(p.group, p.n_groups, r);
+    return p.prefix[g] > 0 ? g : -1;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(FEW_WARPS * 32)
+attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces out)
+{
+    constexpr int CH = HD / 8;                               // 16-byte chunks of a key
+    constexpr int HALF_STAGE = FEW_KEYS * HD * 2, STAGE = 2 * HALF_STAGE;
+    extern __shared__ __align__(128) char smem[];
+    __shared__ long long red[32];
+    __shared__ int red_t[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    Plan p;
+    if (!load_plan(a, p, smem + FEW_WARPS * FEW_STAGES * STAGE, 1)) return;
+    const long long units = lay_line(p, cut, red, red_t);
+    const long long per = stretch(units, out.workers, FEW_LEAST);
+    const int worker = blockIdx.x * FEW_WARPS + warp;
+    long long u = worker * per;
+    const long long u_end = min(units, u + per);
+    if (u >= u_end) return;                                  // warps are independent from here on
+    const uint32_t ring = smem_u32(smem) + warp * FEW_STAGES * STAGE;
+    const uint16_t *kp = static_cast<const uint16_t *>(a.d_k_pool), *vp = static_cast<const uint16_t *>(a.d_v_pool);
+    const float c = a.scale * 1.4426950408889634f;
+    const int sets = p.n_req + p.n_groups, g = lane >> 2, cq = lane & 3;
+    const int page_shift = 31 - __clz(a.page);
+
+    int e = last_at(p.unit, sets, u);
+    while (u < u_end) {
+        while (p.unit[e + 1] <= u) ++e;
+        const Set s = set_at(p, e);
+        const long long head_units = (p.unit[e + 1] - p.unit[e]) / p.n_kv;
+        const int h = (int)((u - p.unit[e]) / head_units), tiles = tiles_of(s, cut);
+        long long rest = u - p.unit[e] - h * head_units;
+        int t = 0, ut = units_of(p, s, cut, 0);
+        while (rest >= ut) { rest -= ut; ++t; ut = units_of(p, s, cut, t); }
+        const int k0 = (int)rest, n = (int)min((long long)(ut - k0), u_end - u);
+        u += n;
+
+        // ---- the piece: query rows t * 16 .. of head h, units k0 .. k0 + n - 1 ----
+        const int row0 = s.own ? p.row[e - p.n_groups] : p.row[p.group[e]], i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
+        const int seen = seen_by(p, s, cut, t), seen_first = s.own ? s.keys - s.rows + i0 / p.G + 1 : s.keys;
+        const int *table = s.own ? a.d_table + (size_t)(e - p.n_groups) * a.table_ld : a.d_prefix_table + (size_t)e * a.prefix_ld;
+        int limit[2];
+        uint32_t q[CH / 2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int i = i0 + g + 8 * half;
+            const bool on = g + 8 * half < valid;
+            limit[half] = !on ? 0 : s.own ? s.keys - s.rows + i / p.G + 1 : s.keys;
+            const uint16_t *src = static_cast<const uint16_t *>(a.d_q) + (long long)(row0 + (on ? i / p.G : 0)) * a.q_ld + (size_t)(h * p.G + (on ? i % p.G : 0)) * HD + 2 * cq;
+#pragma unroll
+            for (int ks = 0; ks < CH / 2; ++ks) {
+                q[ks][half] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * ks) : 0u;
+                q[ks][2 + half] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 8) : 0u;
+            }
+        }
+        int ids = 0;
+        bool outside = false;
+        auto issue = [&](int i) {                            // unit k0 + i of the tile into its place of the ring
+            if (i < n) {
+                if ((i & 31) == 0) {                         // page numbers, 32 units at a time
+                    const int key = (k0 + i + lane) * FEW_KEYS;
+                    ids = i + lane < n ? __ldg(table + (key >> page_shift)) : 0;
+                }
+                const int id = __shfl_sync(0xffffffffu, ids, i & 31), key = (k0 + i) * FEW_KEYS;
+                const bool there = id >= 0 && id < a.n_pages;
+                outside |= !there;
+                const size_t at = (((size_t)(there ? id : 0) * a.n_kv + h) * a.page + (key & (a.page - 1))) * HD;
+                const uint32_t dst = ring + (i % FEW_STAGES) * STAGE;
+#pragma unroll
+                for (int j = 0; j < FEW_KEYS * CH / 32; ++j) {
+                    const int row = (lane + 32 * j) / CH, ch = (lane + 32 * j) % CH;
+                    const bool on = there && key + row < seen;           // what is not seen is not read: zeros
+                    const uint32_t to = dst + row * HD * 2 + ((ch ^ (row & 7)) * 16);
+                    cp16(to, kp + at + (size_t)row * HD + ch * 8, on);
+                    cp16(to + HALF_STAGE, vp + at + (size_t)row * HD + ch * 8, on);
+                }
+            }
+            cp_commit();
+        };
+        float o[CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < CH; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        __syncwarp();                                        // the ring's last reads, of the piece before
+#pragma unroll
+        for (int i = 0; i < FEW_STAGES - 1; ++i) issue(i);
+        for (int i = 0; i < n; ++i) {
+            cp_wait<FEW_STAGES - 2>();
+            __syncwarp();
+            issue(i + FEW_STAGES - 1);
+            const uint32_t kt = ring + (i % FEW_STAGES) * STAGE, vt = kt + HALF_STAGE;
+            const int key = (k0 + i) * FEW_KEYS, mi = lane >> 3, rr = lane & 7;
+            float sc[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < CH / 2; ++ks) {
+                uint32_t b[4];
+                const int row = (mi >> 1) * 8 + rr, ch = ks * 2 + (mi & 1);
+                ldsm4(kt + row * HD * 2 + ((ch ^ (row & 7)) * 16), b);
+                mma16<T>(sc[0], q[ks], b[0], b[1]);
+                mma16<T>(sc[1], q[ks], b[2], b[3]);
+            }
+            float top[2] = {m[0], m[1]};
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = sc[nt][j] * c;
+                    sc[nt][j] = key + nt * 8 + 2 * cq + (j & 1) < limit[j >> 1] ? x : -INFINITY;
+                    top[j >> 1] = fmaxf(top[j >> 1], sc[nt][j]);
+                }
+            float base[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                base[r] = top[r] == -INFINITY ? 0.0f : top[r];
+            }
+            if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+                const float f0 = ex2(m[0] - base[0]), f1 = ex2(m[1] - base[1]);
+                l[0] *= f0; l[1] *= f1;
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) { o[ch][0] *= f0; o[ch][1] *= f0; o[ch][2] *= f1; o[ch][3] *= f1; }
+                m[0] = top[0]; m[1] = top[1];
+            }
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sc[nt][j] = ex2(sc[nt][j] - base[j >> 1]);
+                    l[j >> 1] += sc[nt][j];
+                }
+            if (key + FEW_KEYS > seen_first && seen_first < seen) {
+                // Some rows see keys of this unit that others do not: zero weights must not meet infinities or NaN. Values of such keys are added
+                // row by row where they are seen, and taken out of the product.
+                uint32_t special = 0;
+#pragma unroll 1
+                for (int row = 0; row < FEW_KEYS; ++row) {
+                    const bool mine = lane < CH && any_special<T>(lds_128(vt + row * HD * 2 + (lane % CH) * 16));
+                    if (__any_sync(0xffffffffu, mine)) special |= 1u << row;
+                }
+                while (special) {
+                    const int row = __ffs(special) - 1;
+                    special &= special - 1;
+                    float w[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float even = row < 8 ? sc[0][2 * r] : sc[1][2 * r], odd = row < 8 ? sc[0][2 * r + 1] : sc[1][2 * r + 1];
+                        w[r] = __shfl_sync(0xffffffffu, row & 1 ? odd : even, (lane & ~3) | ((row & 7) >> 1));
+                    }
+#pragma unroll
+                    for (int ch = 0; ch < CH; ++ch) {
+                        uint32_t two;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vt + row * HD * 2 + ((ch ^ (row & 7)) * 16) + 4 * cq));
+                        const float v0 = to_float<T>((uint16_t)two), v1 = to_float<T>((uint16_t)(two >> 16));
+                        if (key + row < limit[0]) { o[ch][0] = fmaf(w[0], v0, o[ch][0]); o[ch][1] = fmaf(w[0], v1, o[ch][1]); }
+                        if (key + row < limit[1]) { o[ch][2] = fmaf(w[1], v0, o[ch][2]); o[ch][3] = fmaf(w[1], v1, o[ch][3]); }
+                    }
+                    __syncwarp();
+                    if (lane < CH) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + row * HD * 2 + lane * 16), "r"(0u) : "memory");
+                    __syncwarp();
+                }
+            }
+            const uint32_t w[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]), pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
+#pragma unroll
+            for (int cp = 0; cp < CH / 2; ++cp) {
+                uint32_t b[4];
+                const int row = (mi & 1) * 8 + rr, ch = cp * 2 + (mi >> 1);
+                ldsm4_t(vt + row * HD * 2 + ((ch ^ (row & 7)) * 16), b);
+                mma16<T>(o[2 * cp], w, b[0], b[1]);
+                mma16<T>(o[2 * cp + 1], w, b[2], b[3]);
+            }
+        }
+        cp_wait<0>();
+        if (outside && lane == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        const bool whole = n == ut && s.own && group_of(p, e - p.n_groups) < 0;          // nothing to join with
+        const long long slot = p.tile[e] + (long long)h * tiles + t + worker;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int k = g + 8 * r, i = i0 + k;
+            if (k >= valid) continue;
+            if (whole) {
+                const float inv = 1.0f / l[r];
+                uint16_t *to = static_cast<uint16_t *>(a.d_out) + (long long)(row0 + i / p.G) * a.out_ld + (size_t)(h * p.G + i % p.G) * HD + 2 * cq;
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) *reinterpret_cast<uint32_t *>(to + 8 * ch) = pack2<T>(o[ch][2 * r] * inv, o[ch][2 * r + 1] * inv);
+            } else {
+                float *to = out.acc + (slot * FEW_ROWS + k) * HD + 2 * cq;
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) *reinterpret_cast<float2 *>(to + 8 * ch) = make_float2(o[ch][2 * r], o[ch][2 * r + 1]);
+                if (cq == 0) out.top[slot * FEW_ROWS + k] = make_float2(m[r], l[r]);
+            }
+        }
+    }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces in)
+{
+    constexpr int N = HD / 32;                               // numbers of a lane, next to one another
+    extern __shared__ __align__(128) char smem[];
+    __shared__ long long red[32];
+    __shared__ int red_t[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    Plan p;
+    if (!load_plan(a, p, smem, 1)) return;
+    const long long units = lay_line(p, cut, red, red_t);
+    const long long per = stretch(units, in.workers, FEW_LEAST);
+    const long long at = (long long)blockIdx.x * JOIN_WARPS + warp;
+    const int row = (int)(at / a.n_q), head = (int)(at % a.n_q);
+    if (row >= p.row[p.n_req]) return;
+    const int r = last_at(p.row, p.n_req, row), h = head / p.G, group = group_of(p, r);
+    long long first[2];                                      // slot and place of the first piece of the prefix and of the own tokens, and how many
+    int count[2] = {0, 0}, place[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        first[k] = 0;
+        const int e = k == 0 ? group : p.n_groups + r;
+        if (e < 0) continue;
+        const Set s = set_at(p, e);
+        if (!in_cut(s, cut)) continue;
+        const int i = (row - (s.own ? p.row[r] : p.row[p.group[e]])) * p.G + head % p.G, t = i / cut.rt;
+        const long long head_units = (p.unit[e + 1] - p.unit[e]) / p.n_kv;
+        const long long b = p.unit[e] + h * head_units + units_before(p, s, cut, t), w0 = b / per, w1 = (b + units_of(p, s, cut, t) - 1) / per;
+        first[k] = p.tile[e] + (long long)h * tiles_of(s, cut) + t + w0;
+        count[k] = (int)(w1 - w0) + 1;
+        place[k] = i % cut.rt;
+    }
+    const int n = count[0] + count[1];
+    if (group < 0 && n == 1) return;                         // stored where it was formed
+    auto where = [&](int j) { return j < count[0] ? (first[0] + j) * cut.rt + place[0] : (first[1] + j - count[0]) * cut.rt + place[1]; };
+    float top = -INFINITY;
+    for (int j = lane; j < n; j += 32) top = fmaxf(top, in.top[where(j)].x);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+        const long long w = where(j);
+        const float2 ml = in.top[w];
+        const float f = ex2(ml.x - base);
+        const float *v = in.acc + w * HD + lane * N;
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(v[i], f, o[i]);
+    }
+    const float inv = 1.0f / l;
+    uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)head * HD + lane * N);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) to[i / 2] = pack2<T>(o[i] * inv, o[i + 1] * inv);
+}
+
+int sm_count()
+{
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    return n;
+}
+
+// Sizes alone: 0, or why they are refused.
+int check_sizes(const b200_paged_attn_args &a)
+{
+    if ((a.wtype != B200_WT_F16 && a.wtype != B200_WT_BF16) || (a.hd != 64 && a.hd != 128 && a.hd != 256)) return B200_E_BADARG;
+    if (a.n_q < 1 || a.n_kv < 1 || a.n_q % a.n_kv || a.n_q > 1024 || a.max_rows < 0 || a.max_rows > (1 << 20) || a.n_pages < 1) return B200_E_BADARG;
+    if (a.page < 16 || a.page > 256 || (a.page & (a.page - 1))) return B200_E_BADARG;
+    if (a.n_req < 0 || a.n_req > B200_PAGED_MAX_REQ || a.n_groups < 0 || a.n_groups > a.n_req) return B200_E_BADARG;
+    if (a.table_ld < 0 || a.table_ld > (1 << 20) || a.prefix_ld < 0 || a.prefix_ld > (1 << 20)) return B200_E_BADARG;
+    if ((long long)a.n_pages * a.page > INT_MAX || (long long)a.table_ld * a.page > INT_MAX || (long long)a.prefix_ld * a.page > INT_MAX) return B200_E_TOOLARGE;
+    return 0;
+}
+
+struct Layout { long long few_workers, few_slots; size_t few_acc, few_top, bytes; };
+
+Layout layout_of(const b200_paged_attn_args &a)
+{
+    const int G = a.n_q / a.n_kv;
+    Layout L = {};
+    L.few_workers = 2LL * sm_count() * FEW_WARPS;
+    // tiles of rows: a part of a tile more for each set that has rows
+    const long long full = ((long long)a.max_rows * G + FEW_ROWS - 1) / FEW_ROWS, sets = (a.n_req < a.max_rows ? a.n_req : a.max_rows) + (a.n_groups < a.max_rows ? a.n_groups : a.max_rows);
+    L.few_slots = (full * (a.n_groups ? 2 : 1) + sets) * a.n_kv + L.few_workers;
+    L.few_acc = 0;
+    L.few_top = L.few_acc + (size_t)L.few_slots * FEW_ROWS * a.hd * 4;
+    L.bytes = L.few_top + (size_t)L.few_slots * FEW_ROWS * 8;
+    return L;
+}
+
+template <typename T, int HD>
+int launch(const b200_paged_attn_args &a, cudaStream_t st)
+{
+    const Layout L = layout_of(a);
+    if (a.work_bytes < L.bytes) return B200_E_BADARG;
+    char *work = static_cast<char *>(a.d_work);
+    const Pieces few = {reinterpret_cast<float *>(work + L.few_acc), reinterpret_cast<float2 *>(work + L.few_top), L.few_workers};
+    const Cut cut = {FEW_ROWS, FEW_KEYS, 0, INT_MAX};
+    const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), smem = (size_t)FEW_WARPS * FEW_STAGES * 2 * FEW_KEYS * HD * 2 + plan;
+    cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(L.few_workers / FEW_WARPS));
+    cfg.blockDim = dim3(FEW_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD>, a, cut, few);
+    if (e != cudaSuccess) return (int)e;
+    ++g_b200_launches;
+    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS)), dim3(JOIN_WARPS * 32), plan, st, a, cut, few);
+    if (e != cudaSuccess) return (int)e;
+    ++g_b200_launches;
+    return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" size_t b200_paged_attn_work_bytes(const b200_paged_attn_args *a)
+{
+    return a && check_sizes(*a) == 0 ? layout_of(*a).bytes : 0;
+}
+
+extern "C" int b200_paged_attn(const b200_paged_attn_args *ap, void *stream)
+{
+    if (!ap) return B200_E_BADARG;
+    const b200_paged_attn_args &a = *ap;
+    if (const int rc = check_sizes(a)) return rc;
+    if (a.max_rows == 0 || a.n_req == 0) return 0;
+    if (!a.d_q || !a.d_k_pool || !a.d_v_pool || !a.d_out || !a.d_row_start || !a.d_len || !a.d_table || !a.d_work) return B200_E_BADARG;
+    if (a.n_groups && (!a.d_group_start || !a.d_prefix_len || (a.prefix_ld && !a.d_prefix_table))) return B200_E_BADARG;
+    if (a.q_ld < (long long)a.n_q * a.hd || a.q_ld % 8 || a.out_ld < (long long)a.n_q * a.hd || a.out_ld % 8) return B200_E_BADARG;
+    if (((uintptr_t)a.d_q | (uintptr_t)a.d_k_pool | (uintptr_t)a.d_v_pool | (uintptr_t)a.d_out | (uintptr_t)a.d_work) % 16) return B200_E_BADARG;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a.wtype == B200_WT_F16) return a.hd == 64 ? launch<__half, 64>(a, st) : a.hd == 128 ? launch<__half, 128>(a, st) : launch<__half, 256>(a, st);
+    return a.hd == 64 ? launch<__nv_bfloat16, 64>(a, st) : a.hd == 128 ? launch<__nv_bfloat16, 128>(a, st) : launch<__nv_bfloat16, 256>(a, st);
+}

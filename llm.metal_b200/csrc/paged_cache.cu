@@ -1,0 +1,294 @@
+// Caches in pages (sm_100a): the tables of a step from the requests' lengths, and the new rows' way into their slots.
+//
+// Tables (extend, release): prefix sums over at most 1024 requests, one a thread, and then one (row or page) a thread, which finds its request by
+// bisection in shared memory. A step of 32 requests is two dependent round trips to L2 and a launch; large ones are stores. One cluster of blocks:
+// all of them scan for themselves, and nothing that was read is written before all have read it, so that lengths and the stack's height
+// can be updated in place. Whole numbers throughout: the same result in every run.
+#include "stream_core.cuh"
+#include "../../include/llmb200_paged_kernels.h"
+
+#include <cuda_bf16.h>
+
+#include <limits.h>
+#include <type_traits>
+
+extern unsigned long long g_b200_launches;
+
+namespace {
+
+// Exclusive sums of x and y over the threads of a block; the totals go to `total`. `red`: 64 ints.
+__device__ __forceinline__ int2 block_scan2(int x, int y, int *red, int2 &total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    int ix = x, iy = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, ix, o), b = __shfl_up_sync(0xffffffffu, iy, o);
+        if (lane >= o) { ix += a; iy += b; }
+    }
+    if (lane == 31) { red[warp] = ix; red[32 + warp] = iy; }
+    __syncthreads();
+    int bx = lane < nw ? red[lane] : 0, by = lane < nw ? red[32 + lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, bx, o), b = __shfl_up_sync(0xffffffffu, by, o);
+        if (lane >= o) { bx += a; by += b; }
+    }
+    total.x = __shfl_sync(0xffffffffu, bx, 31);
+    total.y = __shfl_sync(0xffffffffu, by, 31);
+    const int px = __shfl_sync(0xffffffffu, bx, max(warp - 1, 0)), py = __shfl_sync(0xffffffffu, by, max(warp - 1, 0));
+    return make_int2(ix - x + (warp ? px : 0), iy - y + (warp ? py : 0));
+}
+
+// The last r < n with start[r] <= at (start ascending, start[0] = 0).
+__device__ __forceinline__ int owner_of(const int *start, int n, int at)
+{
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= at) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void report(unsigned *status, unsigned bits)
+{
+    if (status && bits) atomicOr(status, bits);
+}
+
+constexpr int TABLE_BLOCKS = 8;          // a portable cluster
+constexpr int TABLE_ROWS = 2048;         // below this many rows (pages for release) one block does it
+
+template <bool RELEASE>
+__global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b200_pages_args a)
+{
+    __shared__ int s_len[B200_PAGED_MAX_REQ], s_row[B200_PAGED_MAX_REQ], s_page[B200_PAGED_MAX_REQ];
+    __shared__ int red[64];
+    const int r = threadIdx.x, n = a.n_req;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int free_n = *a.d_free_n;
+    int len = 0, rows = 0, pages = 0;
+    unsigned bad = 0;
+    if (r < n) {
+        len = a.d_len[r];
+        const int given = a.d_new[r];
+        const long long room = (long long)a.table_ld * a.page;
+        if (RELEASE) {
+            if (given) {
+                if (len < 0 || len > room) bad = B200_PAGED_BAD_LENGTH;
+                else pages = (len + a.page - 1) / a.page;
+            }
+        } else if (len < 0 || given < 0 || given > a.max_rows || (long long)len + given > room) {
+            bad = B200_PAGED_BAD_LENGTH;
+        } else {
+            rows = given;
+            pages = (len + given + a.page - 1) / a.page - (len + a.page - 1) / a.page;
+        }
+    }
+    int2 total;                                              // at most 1024 * 2^20 each
+    const int2 at = block_scan2(rows, pages, red, total);
+    if (r < n) { s_len[r] = len; s_row[r] = at.x; s_page[r] = at.y; }
+    if (total.x > a.max_rows) bad |= B200_PAGED_BAD_LENGTH;
+    if (free_n < 0 || free_n > a.n_pages || (RELEASE ? free_n + total.y > a.n_pages : total.y > free_n)) bad |= B200_PAGED_NO_PAGES;
+    const unsigned why = (__syncthreads_or(bad & B200_PAGED_BAD_LENGTH) ? B200_PAGED_BAD_LENGTH : 0u) | (__syncthreads_or(bad & B200_PAGED_NO_PAGES) ? B200_PAGED_NO_PAGES : 0u);
+    if (gridDim.x > 1) cluster_sync();                       // all blocks have read what is updated in place
+    if (blockIdx.x == 0) {
+        if (r < n) {
+            a.d_len_out[r] = why ? len : RELEASE ? (a.d_new[r] ? 0 : len) : len + rows;
+            if (!RELEASE) a.d_row_start[r] = why ? 0 : at.x;
+        }
+        if (r == 0) {
+            *a.d_free_n_out = why ? free_n : RELEASE ? free_n + total.y : free_n - total.y;
+            if (!RELEASE) a.d_row_start[n] = why ? 0 : total.x;
+            report(a.d_status, why);
+        }
+    }
+    if (why) return;
+    const int first = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+    for (int p = first; p < total.y; p += step) {
+        const int q = owner_of(s_page, n, p);
+        if (RELEASE) a.d_free[free_n + p] = a.d_table[(size_t)q * a.table_ld + (p - s_page[q])];
+        else a.d_table[(size_t)q * a.table_ld + (s_len[q] + a.page - 1) / a.page + (p - s_page[q])] = a.d_free[free_n - 1 - p];
+    }
+    if (RELEASE) return;
+    unsigned outside = 0;
+    for (int m = first; m < total.x; m += step) {
+        const int q = owner_of(s_row, n, m), token = s_len[q] + (m - s_row[q]), k = token / a.page, held = (s_len[q] + a.page - 1) / a.page;
+        // the pages of this call come from the stack: their numbers in the table may not be there yet
+        const int id = k < held ? a.d_table[(size_t)q * a.table_ld + k] : a.d_free[free_n - 1 - (s_page[q] + k - held)];
+        const bool ok = id >= 0 && id < a.n_pages;
+        a.d_slot[m] = ok ? id * a.page + token % a.page : -1;
+        a.d_pos[m] = (a.d_base ? a.d_base[q] : 0) + token;
+        if (!ok) outside = B200_PAGED_BAD_PAGE;
+    }
+    report(a.d_status, outside);
+}
+
+template <bool RELEASE>
+int launch_pages(const b200_pages_args *ap, void *stream)
+{
+    if (!ap) return B200_E_BADARG;
+    const b200_pages_args &a = *ap;
+    if (a.n_req < 0 || a.n_req > B200_PAGED_MAX_REQ || a.n_pages < 0 || a.table_ld < 0 || a.table_ld > (1 << 20)) return B200_E_BADARG;
+    if (a.page < 16 || a.page > 256 || (a.page & (a.page - 1))) return B200_E_BADARG;
+    if ((long long)a.n_pages * a.page > INT_MAX || (long long)a.table_ld * a.page > INT_MAX) return B200_E_TOOLARGE;
+    if (!a.d_free_n || !a.d_free_n_out || (a.n_req && (!a.d_len || !a.d_len_out || !a.d_new)) || (a.n_req && a.table_ld && !a.d_table) || (a.n_pages && !a.d_free)) return B200_E_BADARG;
+    if (!RELEASE) {
+        if (a.max_rows < 0 || a.max_rows > (1 << 20)) return B200_E_BADARG;
+        if (!a.d_row_start || (a.max_rows && (!a.d_slot || !a.d_pos))) return B200_E_BADARG;
+    }
+    const long long most = RELEASE ? (long long)a.n_req * a.table_ld : a.max_rows;
+    const bool one = most <= TABLE_ROWS;
+    int threads = 1024;
+    if (one) {
+        const int want = a.n_req > (int)most ? a.n_req : (int)most;
+        threads = want >= 1024 ? 1024 : want < 64 ? 64 : (want + 31) & ~31;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(one ? 1 : TABLE_BLOCKS);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = TABLE_BLOCKS; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = one ? 1 : 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_kernel<RELEASE>, a);
+    if (e != cudaSuccess) return (int)e;
+    ++g_b200_launches;
+    return (int)cudaGetLastError();
+}
+
+// ---- new rows into their slots ------------------------------------------------------------------------------------------------
+// Bound by memory: 4 bytes read and 2 written a number. A warp takes a head at a time; its lanes hold the pairs (d, d + hd / 2), so that the norm is a
+// shuffle and the rotation stays in the lane. The angle pos * inv_freq is formed in 64 bits (exact) and brought into one turn before the
+// 32-bit sine and cosine: as a 32-bit product it is off by pos * 2^-24, more than binary16's step from position 8000 on. One a lane pair and
+// block. q, k and v are rounded once, to the type of the cache that the tensor cores read.
+template <typename T> __device__ __forceinline__ uint16_t to_bits(float x)
+{
+    if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rn(x));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+}
+
+template <int N> struct Vec;
+template <> struct Vec<1> { using F = float; using H = uint16_t; };
+template <> struct Vec<2> { using F = float2; using H = uint32_t; };
+template <> struct Vec<4> { using F = float4; using H = uint2; };
+
+constexpr int STORE_WARPS = 8;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __grid_constant__ b200_paged_store_args a, int heads_per_block)
+{
+    constexpr int HALF = HD / 2, N = HALF / 32;              // pairs of a lane
+    using F = typename Vec<N>::F;
+    using H = typename Vec<N>::H;
+    __shared__ float s_cos[HALF], s_sin[HALF];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = blockIdx.x, d = lane * N;
+    pdl_launch_dependents();
+    float gq[2 * N], gk[2 * N];                              // weights: constants, read ahead of the wait
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        gq[j] = a.d_q_gamma ? a.d_q_gamma[d + j] : 1.0f; gq[N + j] = a.d_q_gamma ? a.d_q_gamma[HALF + d + j] : 1.0f;
+        gk[j] = a.d_k_gamma ? a.d_k_gamma[d + j] : 1.0f; gk[N + j] = a.d_k_gamma ? a.d_k_gamma[HALF + d + j] : 1.0f;
+    }
+    const float freq = a.d_inv_freq && threadIdx.x < HALF ? a.d_inv_freq[threadIdx.x] : 0.0f;
+    pdl_wait();
+    if (m >= *a.d_rows) return;
+    if (threadIdx.x < HALF) {
+        constexpr double TURN = 6.283185307179586476925;
+        const double t = (double)a.d_pos[m] * (double)freq;
+        float sn, cs;
+        sincosf((float)(t - rint(t / TURN) * TURN), &sn, &cs);
+        s_cos[threadIdx.x] = cs; s_sin[threadIdx.x] = sn;
+    }
+    const int slot = a.d_slot[m];
+    const bool in_pool = slot >= 0 && slot < a.n_pages * a.page;
+    if (!in_pool && threadIdx.x == 0 && blockIdx.y == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
+    __syncthreads();
+    const int heads = a.n_q + 2 * a.n_kv, h1 = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
+    const float *row = a.d_qkv + (long long)m * a.qkv_ld;
+#pragma unroll 2
+    for (int h = blockIdx.y * heads_per_block + warp; h < h1; h += STORE_WARPS) {
+        float x[2 * N];
+        *reinterpret_cast<F *>(x) = *reinterpret_cast<const F *>(row + h * HD + d);
+        *reinterpret_cast<F *>(x + N) = *reinterpret_cast<const F *>(row + h * HD + HALF + d);
+        if (h < a.n_q + a.n_kv) {
+            const bool is_q = h < a.n_q;
+            if (is_q ? a.d_q_gamma != nullptr : a.d_k_gamma != nullptr) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 2 * N; ++j) ss = fmaf(x[j], x[j], ss);
+                const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.eps);
+#pragma unroll
+                for (int j = 0; j < 2 * N; ++j) x[j] *= (is_q ? gq[j] : gk[j]) * inv;
+            }
+            if (a.d_inv_freq) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float cs = s_cos[d + j], sn = s_sin[d + j], lo = x[j], hi = x[N + j];
+                    x[j] = lo * cs - hi * sn; x[N + j] = lo * sn + hi * cs;
+                }
+            }
+        }
+        uint16_t b[2 * N];
+#pragma unroll
+        for (int j = 0; j < 2 * N; ++j) b[j] = to_bits<T>(x[j]);
+        uint16_t *to;
+        if (h < a.n_q) to = static_cast<uint16_t *>(a.d_q) + (long long)m * a.q_ld + h * HD;
+        else {
+            const int kv = (h - a.n_q) % a.n_kv;
+            if (!in_pool) continue;
+            to = static_cast<uint16_t *>(h < a.n_q + a.n_kv ? a.d_k_pool : a.d_v_pool) + (((long long)(slot / a.page) * a.n_kv + kv) * a.page + slot % a.page) * HD;
+        }
+        H w[2];
+        memcpy(w, b, sizeof(w));
+        *reinterpret_cast<H *>(to + d) = w[0];
+        *reinterpret_cast<H *>(to + HALF + d) = w[1];
+    }
+}
+
+template <typename T>
+int launch_store(const b200_paged_store_args &a, cudaStream_t st)
+{
+    // few rows: a warp to each head, or 32 rows would run on 32 SMs; many: all heads of a row in one block, which forms the angles once
+    const int heads = a.n_q + 2 * a.n_kv, per = a.max_rows <= 512 ? STORE_WARPS : heads;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.max_rows, (heads + per - 1) / per);
+    cfg.blockDim = dim3(STORE_WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = a.hd == 64 ? cudaLaunchKernelEx(&cfg, paged_store_kernel<T, 64>, a, per)
+                        : a.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_store_kernel<T, 128>, a, per) : cudaLaunchKernelEx(&cfg, paged_store_kernel<T, 256>, a, per);
+    if (e != cudaSuccess) return (int)e;
+    ++g_b200_launches;
+    return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" int b200_pages_extend(const b200_pages_args *a, void *stream) { return launch_pages<false>(a, stream); }
+extern "C" int b200_pages_release(const b200_pages_args *a, void *stream) { return launch_pages<true>(a, stream); }
+
+extern "C" int b200_paged_store(const b200_paged_store_args *ap, void *stream)
+{
+    if (!ap) return B200_E_BADARG;
+    const b200_paged_store_args &a = *ap;
+    if ((a.wtype != B200_WT_F16 && a.wtype != B200_WT_BF16) || (a.hd != 64 && a.hd != 128 && a.hd != 256)) return B200_E_BADARG;
+    if (a.n_q < 1 || a.n_kv < 1 || a.n_q % a.n_kv || a.n_q > 1024 || a.max_rows < 0 || a.max_rows > (1 << 20) || a.n_pages < 1) return B200_E_BADARG;
+    if (a.page < 16 || a.page > 256 || (a.page & (a.page - 1))) return B200_E_BADARG;
+    if ((long long)a.n_pages * a.page > INT_MAX) return B200_E_TOOLARGE;
+    if (a.max_rows == 0) return 0;
+    if (!a.d_qkv || !a.d_rows || !a.d_slot || !a.d_pos || !a.d_k_pool || !a.d_v_pool || !a.d_q) return B200_E_BADARG;
+    if (a.qkv_ld < (long long)(a.n_q + 2 * a.n_kv) * a.hd || a.qkv_ld % 4 || a.q_ld < (long long)a.n_q * a.hd || a.q_ld % 8) return B200_E_BADARG;
+    if (((uintptr_t)a.d_qkv | (uintptr_t)a.d_k_pool | (uintptr_t)a.d_v_pool | (uintptr_t)a.d_q | (uintptr_t)a.d_q_gamma | (uintptr_t)a.d_k_gamma | (uintptr_t)a.d_inv_freq) % 16)
+        return B200_E_BADARG;
+    return a.wtype == B200_WT_F16 ? launch_store<__half>(a, (cudaStream_t)stream) : launch_store<__nv_bfloat16>(a, (cudaStream_t)stream);
+}

@@ -1,0 +1,156 @@
+// How the work of attention over pages is cut (sm_100a). The rows of a step meet keys in two kinds of sets: a request's own tokens, which its rows see
+// up to their own place, and a group's prefix, which all rows of the group see whole. A set's query rows -- (row, query head of the key / value head) pairs, in
+// that order -- are cut into tiles of RT, the keys that a tile sees into units of KU, and all units of all sets lie on one line: set after set, and in it
+// key / value head after head, tile after tile. Workers take equal stretches of that line, whatever the lengths are; a tile that the ends of stretches
+// cut leaves pieces -- largest score, sum, weighted sum --, which are joined afterwards. Lengths are known on the device alone, so every block
+// lays out the line for itself: one read of the lengths and a prefix sum, about a microsecond.
+#pragma once
+#include "stream_core.cuh"
+#include "../../include/llmb200_paged_kernels.h"
+
+namespace {
+
+// The sets that a kernel deals with: those of more than `lo` and at most `hi` query rows, in tiles of RT rows and units of KU keys.
+struct Cut { int rt, ku, lo, hi; };
+
+// What a block knows of the step, in shared memory.
+struct Plan {
+    int *row, *len, *group, *prefix;     // [n_req + 1], [n_req], [n_groups + 1], [n_groups]
+    long long *unit;                     // [sets + 1]: units before each set; groups' prefixes first, then requests
+    int *tile;                           // [sets + 1]: (head, tile) pairs before each set
+    int n_req, n_groups, n_kv, G;
+};
+
+__host__ __device__ inline size_t plan_bytes(int n_req, int n_groups, int cuts)
+{
+    const size_t sets = (size_t)n_req + n_groups;
+    const size_t n = (size_t)cuts * ((sets + 1) * 8 + (sets + 2) * 4) + ((size_t)n_req * 2 + 2 + 2 * (size_t)n_groups + 2) * 4;
+    return (n + 15) & ~(size_t)15;
+}
+
+struct Set {
+    int rows, nr, keys;                  // new rows, query rows (rows * G), keys
+    bool own;
+};
+
+__device__ __forceinline__ Set set_at(const Plan &p, int e)
+{
+    Set s;
+    s.own = e >= p.n_groups;
+    if (s.own) {
+        const int r = e - p.n_groups;
+        s.rows = p.row[r + 1] - p.row[r]; s.keys = p.len[r];
+    } else {
+        s.rows = p.row[p.group[e + 1]] - p.row[p.group[e]]; s.keys = p.prefix[e];
+    }
+    s.nr = s.rows * p.G;
+    return s;
+}
+__device__ __forceinline__ bool in_cut(const Set &s, const Cut &c) { return s.nr > c.lo && s.nr <= c.hi && s.keys > 0; }
+__device__ __forceinline__ int tiles_of(const Set &s, const Cut &c) { return (s.nr + c.rt - 1) / c.rt; }
+// keys that the last query row of a tile sees, and the tile's units
+__device__ __forceinline__ int seen_by(const Plan &p, const Set &s, const Cut &c, int t)
+{
+    return s.own ? s.keys - s.rows + (min((t + 1) * c.rt, s.nr) - 1) / p.G + 1 : s.keys;
+}
+__device__ __forceinline__ int units_of(const Plan &p, const Set &s, const Cut &c, int t) { return (seen_by(p, s, c, t) + c.ku - 1) / c.ku; }
+
+__device__ __forceinline__ long long units_before(const Plan &p, const Set &s, const Cut &c, int t)
+{
+    if (!s.own) return (long long)t * units_of(p, s, c, 0);
+    long long n = 0;
+    for (int i = 0; i < t; ++i) n += units_of(p, s, c, i);
+    return n;
+}
+
+// The last e < n with start[e] <= at; start is ascending, start[0] = 0.
+template <typename I> __device__ __forceinline__ int last_at(const I *start, int n, I at)
+{
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= at) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Reads the lengths; false (for the whole block) if one of them does not fit. `mem` holds plan_bytes.
+__device__ inline bool load_plan(const b200_paged_attn_args &a, Plan &p, char *mem, int cuts)
+{
+    const int sets = a.n_req + a.n_groups;
+    p.n_req = a.n_req; p.n_groups = a.n_groups; p.n_kv = a.n_kv; p.G = a.n_q / a.n_kv;
+    p.unit = reinterpret_cast<long long *>(mem);
+    p.tile = reinterpret_cast<int *>(p.unit + (size_t)cuts * (sets + 1));
+    p.row = p.tile + (size_t)cuts * (sets + 2);
+    p.len = p.row + a.n_req + 1;
+    p.group = p.len + a.n_req + 1;
+    p.prefix = p.group + a.n_groups + 1;
+    for (int i = threadIdx.x; i <= a.n_req; i += blockDim.x) {
+        p.row[i] = a.d_row_start[i];
+        if (i < a.n_req) p.len[i] = a.d_len[i];
+    }
+    for (int i = threadIdx.x; i < a.n_groups + (a.n_groups > 0); i += blockDim.x) {
+        p.group[i] = a.d_group_start[i];
+        if (i < a.n_groups) p.prefix[i] = a.d_prefix_len[i];
+    }
+    __syncthreads();
+    int bad = 0;
+    for (int i = threadIdx.x; i < a.n_req; i += blockDim.x) {
+        const int r0 = p.row[i], r1 = p.row[i + 1], len = p.len[i];
+        bad |= (i == 0 && r0 != 0) || r1 < r0 || r1 > a.max_rows;
+        bad |= r1 > r0 && (len < r1 - r0 || len > (long long)a.table_ld * a.page);
+    }
+    for (int i = threadIdx.x; i < a.n_groups; i += blockDim.x) {
+        const int g0 = p.group[i], g1 = p.group[i + 1];
+        bad |= g0 < 0 || g1 < g0 || g1 > a.n_req || p.prefix[i] < 0 || p.prefix[i] > (long long)a.prefix_ld * a.page;
+    }
+    bad = __syncthreads_or(bad);
+    if (bad && blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
+    return !bad;
+}
+
+// Lays the line of one cut. Returns its units. `red`: 32 long longs and 32 ints.
+__device__ inline long long lay_line(Plan &p, const Cut &c, long long *red, int *red_t)
+{
+    const int sets = p.n_req + p.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int each = (sets + blockDim.x - 1) / blockDim.x, e0 = min(sets, (int)threadIdx.x * each), e1 = min(sets, e0 + each);
+    long long u = 0;
+    int t = 0;
+    for (int e = e0; e < e1; ++e) {
+        const Set s = set_at(p, e);
+        long long n = 0;
+        int k = 0;
+        if (in_cut(s, c)) { k = tiles_of(s, c); n = units_before(p, s, c, k) * p.n_kv; k *= p.n_kv; }
+        p.unit[e] = n; p.tile[e] = k;                        // summed up below, by the same thread
+        u += n; t += k;
+    }
+    long long iu = u;
+    int it = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, iu, o);
+        const int y = __shfl_up_sync(0xffffffffu, it, o);
+        if (lane >= o) { iu += x; it += y; }
+    }
+    __syncthreads();                                         // `red` of an earlier line
+    if (lane == 31) { red[warp] = iu; red_t[warp] = it; }
+    __syncthreads();
+    long long all = 0;
+    int all_t = 0;
+    iu -= u; it -= t;
+    for (int w = 0; w < nw; ++w) {
+        if (w == warp) { iu += all; it += all_t; }
+        all += red[w]; all_t += red_t[w];
+    }
+    for (int e = e0; e < e1; ++e) {
+        const long long n = p.unit[e];
+        const int k = p.tile[e];
+        p.unit[e] = iu; p.tile[e] = it;
+        iu += n; it += k;
+    }
+    if (threadIdx.x == 0) { p.unit[sets] = all; p.tile[sets] = all_t; }
+    __syncthreads();
+    return all;
+}
+
+}  // namespace
