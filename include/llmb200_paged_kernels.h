@@ -39,6 +39,7 @@ extern "C" {
 #define B200_PAGED_NO_PAGES   1u   /* extend: fewer free pages than needed; release: more pages than there are */
 #define B200_PAGED_BAD_LENGTH 2u   /* a length, a row count or a range that does not fit its buffer */
 #define B200_PAGED_BAD_PAGE   4u   /* a page number outside the pool */
+#define B200_PAGED_TIMED_OUT  8u   /* a wait inside a kernel ran out: the call's results are invalid */
 
 /* ------------------------------------------------------------------------
  * b200_pages_extend: request r holds d_len[r] tokens of its own and takes d_new[r] more (0: none). It gets the pages that

@@ -21,7 +21,7 @@ c_u32_p = C.POINTER(C.c_uint32)
 
 B200_MAX_PEERS = 8
 B200_WT_Q8, B200_WT_F16, B200_WT_BF16, B200_WT_F32 = 0, 1, 2, 3
-B200_PAGED_MAX_REQ, B200_PAGED_NO_PAGES, B200_PAGED_BAD_LENGTH, B200_PAGED_BAD_PAGE = 1024, 1, 2, 4
+B200_PAGED_MAX_REQ, B200_PAGED_NO_PAGES, B200_PAGED_BAD_LENGTH, B200_PAGED_BAD_PAGE, B200_PAGED_TIMED_OUT = 1024, 1, 2, 4, 8
 B200_IN_VEC, B200_IN_RESID, B200_IN_EMBED, B200_IN_POSTNORM = 0, 1, 2, 3
 B200_OUT_STORE, B200_OUT_GLU, B200_OUT_GATED, B200_OUT_STREAMS = 0, 1, 2, 3
 B200_ACT_SILU, B200_ACT_GELU_TANH, B200_ACT_RELU2 = 0, 1, 2

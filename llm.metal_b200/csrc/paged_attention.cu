@@ -7,14 +7,7 @@
 // no barrier in the loop. Scores, maxima, sums and results are fp32; weights are rounded to the cache's type for the second product, by at most
 // half a step each, which is what the results' own rounding is.
 // attn_join_kernel: a warp to each (row, query head) whose keys were cut, over the pieces in the order of the line.
-#include "paged_plan.cuh"
-
-#include <cuda_bf16.h>
-
-#include <limits.h>
-#include <type_traits>
-
-extern unsigned long long g_b200_launches;
+#include "paged_attention.cuh"
 
 namespace {
 
@@ -35,13 +28,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-__device__ __forceinline__ float ex2(float x)                // 2^x, 2 ulp, 0 for -inf
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     if constexpr (std::is_same<T, __half>::value)
@@ -51,54 +37,9 @@ template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-}
-template <typename T> __device__ __forceinline__ float to_float(uint16_t b)
-{
-    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(b));
-    else return __uint_as_float((uint32_t)b << 16);
-}
-// Whether one of the eight elements of a 16-byte word is infinite or NaN.
-template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v)
-{
-    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
-    return any;
-}
-
-// Where a kernel's pieces lie in d_work: [slot][rt][hd] sums and [slot][rt] (largest score, sum). A tile's piece of worker w is in slot tile + w: the
-// number of a piece never falls from one to the next on the line and one of the two grows.
-struct Pieces { float *acc; float2 *top; long long workers; };
-
-// Units of a worker: equal stretches, and none so short that joining costs more than it spreads.
-__device__ __forceinline__ long long stretch(long long units, long long workers, int least)
-{
-    const long long per = (units + workers - 1) / workers;
-    return per < least ? least : per;
-}
-
-// Whether the rows of a request have keys in a prefix.
-__device__ __forceinline__ int group_of(const Plan &p, int r)
-{
-    if (!p.n_groups || r < p.group[0] || r >= p.group[p.n_groups]) return -1;
-    const int g = last_at(p.group, p.n_groups, r);
-    return p.prefix[g] > 0 ? g : -1;
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
-attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces out)
+attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces out, int beside)
 {
     constexpr int CH = HD / 8;                               // 16-byte chunks of a key
     constexpr int HALF_STAGE = FEW_KEYS * HD * 2, STAGE = 2 * HALF_STAGE;
@@ -107,37 +48,28 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
     __shared__ int red_t[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_launch_dependents();
-    pdl_wait();
+    // Beside attn_many_kernel, launched before: its blocks let this grid start when they have waited for what came before, so that everything that is read here
+    // is there. Its results are waited for at the end, for the join's sake, whose own wait covers this grid alone.
+    if (!beside) pdl_wait();
     Plan p;
-    if (!load_plan(a, p, smem + FEW_WARPS * FEW_STAGES * STAGE, 1)) return;
-    const long long units = lay_line(p, cut, red, red_t);
-    const long long per = stretch(units, out.workers, FEW_LEAST);
+    if (!load_plan(a, p, smem + FEW_WARPS * FEW_STAGES * STAGE, 1)) { pdl_wait(); return; }
+    const Line line = lay_line(p, cut, 0, out.workers, red, red_t);
     const int worker = blockIdx.x * FEW_WARPS + warp;
-    long long u = worker * per;
-    const long long u_end = min(units, u + per);
-    if (u >= u_end) return;                                  // warps are independent from here on
     const uint32_t ring = smem_u32(smem) + warp * FEW_STAGES * STAGE;
     const uint16_t *kp = static_cast<const uint16_t *>(a.d_k_pool), *vp = static_cast<const uint16_t *>(a.d_v_pool);
     const float c = a.scale * 1.4426950408889634f;
-    const int sets = p.n_req + p.n_groups, g = lane >> 2, cq = lane & 3;
+    const int g = lane >> 2, cq = lane & 3;
     const int page_shift = 31 - __clz(a.page);
 
-    int e = last_at(p.unit, sets, u);
-    while (u < u_end) {
-        while (p.unit[e + 1] <= u) ++e;
-        const Set s = set_at(p, e);
-        const long long head_units = (p.unit[e + 1] - p.unit[e]) / p.n_kv;
-        const int h = (int)((u - p.unit[e]) / head_units), tiles = tiles_of(s, cut);
-        long long rest = u - p.unit[e] - h * head_units;
-        int t = 0, ut = units_of(p, s, cut, 0);
-        while (rest >= ut) { rest -= ut; ++t; ut = units_of(p, s, cut, t); }
-        const int k0 = (int)rest, n = (int)min((long long)(ut - k0), u_end - u);
-        u += n;
-
-        // ---- the piece: query rows t * 16 .. of head h, units k0 .. k0 + n - 1 ----
-        const int row0 = s.own ? p.row[e - p.n_groups] : p.row[p.group[e]], i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
+    Walk walk(p, line, worker);                              // warps are independent from here on
+    Piece piece;
+    while (walk.next(p, line, cut, piece)) {
+        // ---- query rows t * 16 .. of head h, units k0 .. k0 + n - 1 ----
+        const Set &s = piece.s;
+        const int e = piece.e, h = piece.h, t = piece.t, k0 = piece.k0, n = piece.n;
+        const int row0 = first_row(p, piece), i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
         const int seen = seen_by(p, s, cut, t), seen_first = s.own ? s.keys - s.rows + i0 / p.G + 1 : s.keys;
-        const int *table = s.own ? a.d_table + (size_t)(e - p.n_groups) * a.table_ld : a.d_prefix_table + (size_t)e * a.prefix_ld;
+        const int *table = pages_of(a, piece);
         int limit[2];
         uint32_t q[CH / 2][4];
 #pragma unroll
@@ -275,8 +207,8 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
-        const bool whole = n == ut && s.own && group_of(p, e - p.n_groups) < 0;          // nothing to join with
-        const long long slot = p.tile[e] + (long long)h * tiles + t + worker;
+        const bool whole = n == piece.ut && s.own && group_of(p, e - p.n_groups) < 0;          // nothing to join with
+        const long long slot = line.tile[e] + (long long)h * piece.tiles + t + worker;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int k = g + 8 * r, i = i0 + k;
@@ -294,11 +226,12 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
             }
         }
     }
+    pdl_wait();
 }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces in)
+attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut0, const Pieces in0, const Cut cut1, const Pieces in1)
 {
     constexpr int N = HD / 32;                               // numbers of a lane, next to one another
     extern __shared__ __align__(128) char smem[];
@@ -308,34 +241,44 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, 
     pdl_launch_dependents();
     pdl_wait();
     Plan p;
-    if (!load_plan(a, p, smem, 1)) return;
-    const long long units = lay_line(p, cut, red, red_t);
-    const long long per = stretch(units, in.workers, FEW_LEAST);
+    if (!load_plan(a, p, smem, 2)) return;
+    const Line few = lay_line(p, cut0, 0, in0.workers, red, red_t), many = lay_line(p, cut1, 1, in1.workers, red, red_t);
     const long long at = (long long)blockIdx.x * JOIN_WARPS + warp;
     const int row = (int)(at / a.n_q), head = (int)(at % a.n_q);
     if (row >= p.row[p.n_req]) return;
     const int r = last_at(p.row, p.n_req, row), h = head / p.G, group = group_of(p, r);
-    long long first[2];                                      // slot and place of the first piece of the prefix and of the own tokens, and how many
-    int count[2] = {0, 0}, place[2] = {0, 0};
+    // the row's pieces of the prefix and of the own tokens: where the first one lies, how many, how far apart
+    const float *acc[2] = {};
+    const float2 *tops[2] = {};
+    int count[2] = {0, 0}, step[2] = {0, 0};
+    bool cut_up = false;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        first[k] = 0;
         const int e = k == 0 ? group : p.n_groups + r;
         if (e < 0) continue;
         const Set s = set_at(p, e);
-        if (!in_cut(s, cut)) continue;
-        const int i = (row - (s.own ? p.row[r] : p.row[p.group[e]])) * p.G + head % p.G, t = i / cut.rt;
-        const long long head_units = (p.unit[e + 1] - p.unit[e]) / p.n_kv;
-        const long long b = p.unit[e] + h * head_units + units_before(p, s, cut, t), w0 = b / per, w1 = (b + units_of(p, s, cut, t) - 1) / per;
-        first[k] = p.tile[e] + (long long)h * tiles_of(s, cut) + t + w0;
-        count[k] = (int)(w1 - w0) + 1;
-        place[k] = i % cut.rt;
+        const bool is_few = in_cut(s, cut0);
+        const Cut &cut = is_few ? cut0 : cut1;
+        const Line &line = is_few ? few : many;
+        const Pieces &in = is_few ? in0 : in1;
+        const int i = (row - (s.own ? p.row[r] : p.row[p.group[e]])) * p.G + head % p.G, t = i / cut.rt, tiles = tiles_of(s, cut);
+        const long long head_units = (line.unit[e + 1] - line.unit[e]) / p.n_kv;
+        const long long b = line.unit[e] + h * head_units + units_before(p, s, cut, t), w0 = b / line.per, w1 = (b + units_of(p, s, cut, t) - 1) / line.per;
+        // a tile of 128 rows at most, in places for 256: two pieces in each, of every other unit
+        const bool halves = !is_few && s.nr - t * MANY_ROWS <= MANY_ROWS / 2;
+        const long long place = (line.tile[e] + (long long)h * tiles + t + w0) * cut.rt + i % cut.rt;
+        acc[k] = in.acc + place * HD;
+        tops[k] = in.top + place;
+        step[k] = halves ? cut.rt / 2 : cut.rt;
+        count[k] = (int)(w1 - w0 + 1) * (halves ? 2 : 1);
+        cut_up |= w1 > w0 || halves;
     }
     const int n = count[0] + count[1];
-    if (group < 0 && n == 1) return;                         // stored where it was formed
-    auto where = [&](int j) { return j < count[0] ? (first[0] + j) * cut.rt + place[0] : (first[1] + j - count[0]) * cut.rt + place[1]; };
+    if (group < 0 && !cut_up) return;                        // stored where it was formed
+    auto top_of = [&](int j) { return j < count[0] ? tops[0][(long long)j * step[0]] : tops[1][(long long)(j - count[0]) * step[1]]; };
+    auto acc_of = [&](int j) { return j < count[0] ? acc[0] + (long long)j * step[0] * HD : acc[1] + (long long)(j - count[0]) * step[1] * HD; };
     float top = -INFINITY;
-    for (int j = lane; j < n; j += 32) top = fmaxf(top, in.top[where(j)].x);
+    for (int j = lane; j < n; j += 32) top = fmaxf(top, top_of(j).x);
     top = warp_max(top);
     const float base = top == -INFINITY ? 0.0f : top;
     float l = 0.0f, o[N];
@@ -343,10 +286,9 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, 
     for (int i = 0; i < N; ++i) o[i] = 0.0f;
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
-        const long long w = where(j);
-        const float2 ml = in.top[w];
+        const float2 ml = top_of(j);
         const float f = ex2(ml.x - base);
-        const float *v = in.acc + w * HD + lane * N;
+        const float *v = acc_of(j) + lane * N;
         l = fmaf(ml.y, f, l);
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = fmaf(v[i], f, o[i]);
@@ -372,23 +314,33 @@ int check_sizes(const b200_paged_attn_args &a)
     if (a.page < 16 || a.page > 256 || (a.page & (a.page - 1))) return B200_E_BADARG;
     if (a.n_req < 0 || a.n_req > B200_PAGED_MAX_REQ || a.n_groups < 0 || a.n_groups > a.n_req) return B200_E_BADARG;
     if (a.table_ld < 0 || a.table_ld > (1 << 20) || a.prefix_ld < 0 || a.prefix_ld > (1 << 20)) return B200_E_BADARG;
-    if ((long long)a.n_pages * a.page > INT_MAX || (long long)a.table_ld * a.page > INT_MAX || (long long)a.prefix_ld * a.page > INT_MAX) return B200_E_TOOLARGE;
+    if ((long long)a.n_pages * a.page > INT_MAX || (long long)a.n_pages * a.n_kv > INT_MAX || (long long)a.table_ld * a.page > INT_MAX || (long long)a.prefix_ld * a.page > INT_MAX) return B200_E_TOOLARGE;
     return 0;
 }
 
-struct Layout { long long few_workers, few_slots; size_t few_acc, few_top, bytes; };
+// Sets of more query rows than this go to attn_many_kernel, where hd is one of its own.
+constexpr int FEW_MOST = 16;
+
+struct Layout { long long few_workers, many_workers; size_t few_acc, few_top, many_acc, many_top, bytes; };
 
 Layout layout_of(const b200_paged_attn_args &a)
 {
-    const int G = a.n_q / a.n_kv;
+    const long long G = a.n_q / a.n_kv, all = a.max_rows * G * (a.n_groups ? 2 : 1);         // query rows of all sets
+    const long long sets = (a.n_req < a.max_rows ? a.n_req : a.max_rows) + (a.n_groups < a.max_rows ? a.n_groups : a.max_rows);
     Layout L = {};
     L.few_workers = 2LL * sm_count() * FEW_WARPS;
-    // tiles of rows: a part of a tile more for each set that has rows
-    const long long full = ((long long)a.max_rows * G + FEW_ROWS - 1) / FEW_ROWS, sets = (a.n_req < a.max_rows ? a.n_req : a.max_rows) + (a.n_groups < a.max_rows ? a.n_groups : a.max_rows);
-    L.few_slots = (full * (a.n_groups ? 2 : 1) + sets) * a.n_kv + L.few_workers;
+    L.many_workers = a.hd <= 128 && all > FEW_MOST ? sm_count() : 0;
+    // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
+    const long long few_most = L.many_workers ? FEW_MOST : all;
+    const long long few_tiles = sets * ((few_most + FEW_ROWS - 1) / FEW_ROWS), full = (all + FEW_ROWS - 1) / FEW_ROWS + sets;
+    const long long few_slots = (few_tiles < full ? few_tiles : full) * a.n_kv + L.few_workers;
+    const long long many_sets = all / (FEW_MOST + 1) < sets ? all / (FEW_MOST + 1) : sets;
+    const long long many_slots = L.many_workers ? ((all + MANY_ROWS - 1) / MANY_ROWS + many_sets) * a.n_kv + L.many_workers : 0;
     L.few_acc = 0;
-    L.few_top = L.few_acc + (size_t)L.few_slots * FEW_ROWS * a.hd * 4;
-    L.bytes = L.few_top + (size_t)L.few_slots * FEW_ROWS * 8;
+    L.few_top = L.few_acc + (size_t)few_slots * FEW_ROWS * a.hd * 4;
+    L.many_acc = L.few_top + (size_t)few_slots * FEW_ROWS * 8;
+    L.many_top = L.many_acc + (size_t)many_slots * MANY_ROWS * a.hd * 4;
+    L.bytes = L.many_top + (size_t)many_slots * MANY_ROWS * 8;
     return L;
 }
 
@@ -399,7 +351,11 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     if (a.work_bytes < L.bytes) return B200_E_BADARG;
     char *work = static_cast<char *>(a.d_work);
     const Pieces few = {reinterpret_cast<float *>(work + L.few_acc), reinterpret_cast<float2 *>(work + L.few_top), L.few_workers};
-    const Cut cut = {FEW_ROWS, FEW_KEYS, 0, INT_MAX};
+    const Pieces many = {reinterpret_cast<float *>(work + L.many_acc), reinterpret_cast<float2 *>(work + L.many_top), L.many_workers};
+    const Cut few_cut = {FEW_ROWS, FEW_KEYS, 0, L.many_workers ? FEW_MOST : INT_MAX, FEW_LEAST};
+    const Cut many_cut = {MANY_ROWS, MANY_KEYS, L.many_workers ? FEW_MOST : INT_MAX, INT_MAX, MANY_LEAST};
+    if (L.many_workers)
+        if (const int rc = attn_many_launch(a, many_cut, many, st)) return rc;
     const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), smem = (size_t)FEW_WARPS * FEW_STAGES * 2 * FEW_KEYS * HD * 2 + plan;
     cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
@@ -410,13 +366,16 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
+    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0 || L.many_workers;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD>, a, cut, few);
+    e = cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD>, a, few_cut, few, (int)(L.many_workers != 0));
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
-    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS)), dim3(JOIN_WARPS * 32), plan, st, a, cut, few);
+    const size_t both = plan_bytes(a.n_req, a.n_groups, 2);
+    if (both > 48 * 1024 && (e = cudaFuncSetAttribute(attn_join_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)both)) != cudaSuccess) return (int)e;
+    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS)), dim3(JOIN_WARPS * 32), both, st, a, few_cut, few,
+                       many_cut, many);
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
     return (int)cudaGetLastError();

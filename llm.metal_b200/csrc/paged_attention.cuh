@@ -1,0 +1,52 @@
+// What the two forms of attention over pages share: elements of the cache's type, and the second form's launch.
+#pragma once
+#include "paged_plan.cuh"
+
+#include <cuda_bf16.h>
+
+#include <limits.h>
+#include <type_traits>
+
+extern unsigned long long g_b200_launches;
+
+namespace {
+
+__device__ __forceinline__ float ex2(float x)                // 2^x, 2 ulp, 0 for -inf
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <typename T> __device__ __forceinline__ float to_float(uint16_t b)
+{
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(b));
+    else return __uint_as_float((uint32_t)b << 16);
+}
+// Whether one of the eight elements of a 16-byte word is infinite or NaN.
+template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v)
+{
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || ((w[i] >> 16) & E) == E;
+    return any;
+}
+
+constexpr int MANY_ROWS = 256, MANY_KEYS = 128, MANY_LEAST = 2;
+
+}  // namespace
+
+// attn_many_kernel (paged_attention_many.cu): the sets of more than `lo` query rows, hd 64 or 128. One block to an SM.
+int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st);

@@ -1,0 +1,518 @@
+// Attention over pages for sets of many query rows (sm_100a): the prefix that a group shares, and the own tokens of requests that bring portions of prompts
+// (paged_plan.cuh). Both products run on tcgen05.
+//
+// A block works on two streams that take turns on the tensor core, so that one's softmax runs under the other's products: the two halves of a tile of 256 query
+// rows on the same keys, or, where a tile has 128 rows at most, the same rows on every other unit of 128 keys, each stream with a maximum, sum and result of its own.
+// Per unit and stream: S = Q K^T (128 x 128, tensor memory), the weights P = 2^(c S - m) back into S's place as 16-bit pairs, O += P V with P as the operand from
+// tensor memory and V as it lies, [key][hd] (the product's second operand along its rows). m is the largest score so far only as far as it must be: O is rescaled when it
+// is exceeded by a factor of 2^8, which both 16-bit types have room for.
+//   warp 0      pages into a ring of shared memory: TMA, a box of 64 numbers by up to 128 tokens a lane, keys and values by turns
+//   warp 1      one lane issues the products
+//   warps 4-7   stream 0: queries into shared memory, softmax, results; warps 8-11 stream 1. A thread to a row.
+// Bound by memory for one tile of rows to a set (decode of a group), by the tensor core and the exponentials for several.
+// Every wait is bounded; on a timeout the block reports it, lets copies in flight land, frees its tensor memory and returns.
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+constexpr int MANY_THREADS = 384, HALF_ROWS = MANY_ROWS / 2, MOST_SLOTS = 8;
+constexpr uint32_t BLOCK64 = MANY_KEYS * 128;                // 128 rows of 64 numbers
+constexpr int S_COL = 0, O_COL = 256;                        // tensor memory: S of stream s at 128 s, O at 256 + 128 s
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+// Second operand that lies along its rows ([k][n], 128-byte swizzle): 8 rows of k 1024 bytes apart, 64 columns of n `block` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t block)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// first operand from tensor memory
+__device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) { tmem_st16(taddr, r); tmem_st16(taddr + 16, r + 16); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr)
+{
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    return r;
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t swizzled(int row, int ch) { return (ch >> 3) * BLOCK64 + row * 128 + (((ch & 7) ^ (row & 7)) * 16); }     // chunk ch of a row
+__device__ __forceinline__ void zero16(uint32_t at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory"); }
+
+// The rows' results plus weight times value of one key, for rows that see it: by the whole warp.
+template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at, uint32_t o_at, uint32_t v_at, int key, bool sees)
+{
+    const uint32_t two = tmem_ld1(s_at + key / 2);
+    const float e = to_float<T>((uint16_t)(key & 1 ? two >> 16 : two));
+#pragma unroll 1
+    for (int k = 0; k < HD; k += 32) {
+        uint32_t x[32];
+        tmem_ld32(o_at + k, x);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+            const uint4 v = lds_128(v_at + swizzled(key, k / 8 + ch));
+            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float a = __uint_as_float(x[8 * ch + 2 * q]), b = __uint_as_float(x[8 * ch + 2 * q + 1]);
+                x[8 * ch + 2 * q] = __float_as_uint(sees ? fmaf(e, to_float<T>((uint16_t)word[q]), a) : a);
+                x[8 * ch + 2 * q + 1] = __float_as_uint(sees ? fmaf(e, to_float<T>((uint16_t)(word[q] >> 16)), b) : b);
+            }
+        }
+        tmem_st32(o_at + k, x);
+    }
+    tmem_wait_st();
+}
+
+struct ManyArgs { int slots, plan_off; };
+
+// Which units of a piece a stream has.
+struct Streams {
+    bool halves;                         // one tile of rows, every other unit to a stream
+    int units[2];
+};
+__device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q)
+{
+    Streams w;
+    const int valid = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS);
+    w.halves = valid <= HALF_ROWS;
+    if (w.halves) { w.units[0] = (q.n + 1) / 2; w.units[1] = q.n / 2; return w; }
+    const int seen = q.s.own ? q.s.keys - q.s.rows + (q.t * MANY_ROWS + HALF_ROWS - 1) / p.G + 1 : q.s.keys;
+    w.units[0] = max(0, min(q.n, (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
+    w.units[1] = q.n;
+    return w;
+}
+// The order in which keys and values of a piece of n units pass through the ring: K0 V0 K1 V1 .. for two halves of rows; K0 K1 V0 K2 V1 K3 .. for every other unit.
+__device__ __forceinline__ int place_of_values(bool halves, int n, int j) { return halves ? 2 + j + min(j, n - 2) : 2 * j + 1; }
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ b200_paged_attn_args a, const Cut cut,
+                 const Pieces out, const ManyArgs m)
+{
+    constexpr int NB = HD / 64;
+    constexpr uint32_t SLOT = BLOCK64 * NB, Q_TILE = BLOCK64 * NB;
+    constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(MANY_KEYS >> 3) << 17) | (8u << 24);
+    constexpr uint32_t IDESC_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
+    extern __shared__ __align__(1024) char smem[];
+    __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2], p_bar[2], o_bar[2], alone_bar[2], both_bar;
+    __shared__ long long red[32];
+    __shared__ int red_t[32];
+    __shared__ uint32_t tmem_sh;
+    __shared__ int abort_sh;
+    __shared__ uint32_t special_sh[4][4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort_flag = &abort_sh;
+    char *base = smem + ((1024 - (smem_u32(smem) & 1023)) & 1023);
+    const uint32_t q_tiles = smem_u32(base), ring = q_tiles + 2 * Q_TILE;
+
+    if (threadIdx.x == 0) {
+        abort_sh = 0;
+        for (int s = 0; s < m.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_bar[s], 128); mbar_init(&s_bar[s], 1); mbar_init(&p_bar[s], 128); mbar_init(&o_bar[s], 1); mbar_init(&alone_bar[s], 128);
+        }
+        mbar_init(&both_bar, 256);
+        for (int i = 0; i < 16; ++i) special_sh[i >> 2][i & 3] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tmem = tmem_sh;
+    pdl_wait();
+    pdl_launch_dependents();                                 // after the wait: attn_few_kernel starts on this and waits for nothing else
+    Plan p;
+    const bool fits = load_plan(a, p, base + m.plan_off, 1);
+    Line line = {};
+    if (fits) line = lay_line(p, cut, 0, out.workers, red, red_t);
+    Walk walk(p, line, fits ? blockIdx.x : 0);
+    Piece piece;
+    auto give_up = [&]() { if (!*abort_flag) { *abort_flag = 1; if (a.d_status) atomicOr(a.d_status, B200_PAGED_TIMED_OUT); } };
+
+    if (warp == 0) {
+        // ---- pages into the ring ----
+        const int box = min(a.page, MANY_KEYS), page_shift = 31 - __clz(a.page), boxes = MANY_KEYS / box;
+        asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
+        uint32_t item = 0;
+        bool outside = false, ok = true;
+        while (ok && walk.next(p, line, cut, piece)) {
+            const Streams w = streams_of(p, piece);
+            const int *table = pages_of(a, piece);
+            const int seen = seen_by(p, piece.s, cut, piece.t), n = piece.n;
+            auto load = [&](int unit, bool values) {         // by the whole warp
+                const int slot = item % m.slots;
+                const uint32_t phase = (item / m.slots) & 1;
+                ++item;
+                const int key0 = (piece.k0 + unit) * MANY_KEYS, there = min(boxes, (seen - key0 + box - 1) / box);
+                const int mine = lane / NB, part = lane % NB, key = key0 + mine * box;
+                int id = mine < there ? __ldg(table + (key >> page_shift)) : 0;
+                if (id < 0 || id >= a.n_pages) { outside = true; id = -1; }
+                if (!__all_sync(0xffffffffu, wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag))) { ok = false; return; }
+                if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)there * box * 128 * NB);
+                __syncwarp();
+                if (mine < there)                            // an id of -1 is outside the map and reads as zeros
+                    tma_load_3d(ring + slot * SLOT + part * BLOCK64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
+                                id < 0 ? -1 : id * a.n_kv + piece.h, &full_bar[slot]);
+            };
+            if (w.halves) {
+                load(0, false);
+                if (ok && n > 1) load(1, false);
+                for (int j = 0; j < n && ok; ++j) {
+                    load(j, true);
+                    if (ok && j + 2 < n) load(j + 2, false);
+                }
+            } else {
+                for (int j = 0; j < n && ok; ++j) {
+                    load(j, false);
+                    if (ok) load(j, true);
+                }
+            }
+        }
+        if (!ok) give_up();
+        if (outside && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
+    } else if (warp == 1) {
+        // ---- the products ----
+        if (lane == 0) {
+            uint32_t item = 0, turn = 0, p_phase[2] = {0, 0};
+            bool ok = true;
+            auto full = [&](uint32_t i) {
+                if (ok && !wait_or_abort(&full_bar[i % m.slots], (i / m.slots) & 1, abort_flag)) ok = false;
+                after_sync();
+            };
+            auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % m.slots]); };
+            while (ok && walk.next(p, line, cut, piece)) {
+                const Streams w = streams_of(p, piece);
+                const int n = piece.n;
+                for (int s = 0; s < 2 && ok; ++s) ok = wait_or_abort(&q_bar[s], turn & 1, abort_flag);
+                ++turn;
+                if (!ok) break;
+                after_sync();
+                auto scores = [&](int s, uint32_t i) {
+                    const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % m.slots) * SLOT;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint64_t qd = smem_desc_sw128(q + b * BLOCK64), kd = smem_desc_sw128(k + b * BLOCK64);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) umma_f16(tmem + S_COL + s * 128, qd + 2 * j, kd + 2 * j, IDESC_S, (b | j) != 0);
+                    }
+                    umma_commit(&s_bar[s]);
+                };
+                auto sums = [&](int s, uint32_t i) {
+                    if (!wait_or_abort(&p_bar[s], p_phase[s], abort_flag)) { ok = false; return; }
+                    p_phase[s] ^= 1;
+                    after_sync();
+                    const uint64_t vd = smem_desc_rows(ring + (i % m.slots) * SLOT, BLOCK64);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) umma_from_tmem(tmem + O_COL + s * 128, tmem + S_COL + s * 128 + 8 * j, vd + 128 * j, IDESC_O);
+                };
+                if (w.halves) {
+                    full(item);
+                    if (!ok) break;
+                    scores(0, item); release(item);
+                    if (n > 1) { full(item + 1); if (!ok) break; scores(1, item + 1); release(item + 1); }
+                    else umma_commit(&o_bar[1]);
+                    for (int j = 0; j < n && ok; ++j) {
+                        const uint32_t v = item + place_of_values(true, n, j);
+                        full(v);
+                        if (ok) sums(j & 1, v);
+                        if (!ok) break;
+                        release(v);
+                        if (j + 2 < n) { full(v + 1); if (!ok) break; scores(j & 1, v + 1); release(v + 1); }
+                        else umma_commit(&o_bar[j & 1]);
+                    }
+                } else {
+                    full(item);
+                    if (!ok) break;
+                    if (w.units[0] > 0) scores(0, item); else umma_commit(&o_bar[0]);
+                    scores(1, item); release(item);
+                    for (int j = 0; j < n && ok; ++j) {
+                        const uint32_t v = item + 2 * j + 1;
+                        full(v);
+                        if (ok && j < w.units[0]) {
+                            sums(0, v);
+                            if (!ok) break;
+                            if (j + 1 < w.units[0]) { full(v + 1); if (!ok) break; scores(0, v + 1); } else umma_commit(&o_bar[0]);
+                        }
+                        if (ok) sums(1, v);
+                        if (!ok) break;
+                        release(v);
+                        if (j + 1 < n) { full(v + 1); if (!ok) break; scores(1, v + 1); release(v + 1); } else umma_commit(&o_bar[1]);
+                    }
+                }
+                item += 2 * n;
+            }
+            if (!ok) give_up();
+        }
+    } else if (warp >= 4) {
+        // ---- a stream's rows ----
+        const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;       // stream, row of its tile = lane of tensor memory
+        const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), s_at = tm + S_COL + s * 128, o_at = tm + O_COL + s * 128;
+        const float c = fabsf(a.scale) * 1.4426950408889634f;            // the sign goes into the queries
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        uint32_t turn = 0, item = 0, s_phase = 0, alone_phase = 0, both_phase = 0;
+        bool ok = true;
+        while (ok && walk.next(p, line, cut, piece)) {
+            const Streams w = streams_of(p, piece);
+            const Set &st = piece.s;
+            const int i0 = piece.t * MANY_ROWS, i = i0 + (w.halves ? 0 : s * HALF_ROWS) + r, row0 = first_row(p, piece);
+            const bool valid = i < st.nr;
+            const int seen = seen_by(p, st, cut, piece.t), mine = w.units[s];
+            // keys that this row sees, that the first row of the whole tile sees (all rows see), and the first one of this warp
+            const int limit = st.own ? st.keys - st.rows + min(i, st.nr - 1) / p.G + 1 : st.keys;
+            const int limit_all = st.own ? st.keys - st.rows + i0 / p.G + 1 : st.keys, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
+            const bool warp_valid = __any_sync(0xffffffffu, valid);
+            if (valid && !(w.halves && s == 1)) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.d_q) + (long long)(row0 + i / p.G) * a.q_ld + (size_t)(piece.h * p.G + i % p.G) * HD);
+                const uint32_t dst = q_tiles + s * Q_TILE;
+#pragma unroll
+                for (int ch = 0; ch < HD / 8; ++ch) {
+                    const uint4 v = src[ch];
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + swizzled(r, ch)), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip),
+                                 "r"(v.w ^ flip) : "memory");
+                }
+            }
+            async_proxy_fence();
+            {
+                uint32_t zero[32] = {};
+#pragma unroll
+                for (int k = 0; k < HD; k += 32) tmem_st32(o_at + k, zero);
+                tmem_wait_st();
+            }
+            before_sync();
+            mbar_arrive(&q_bar[s]);
+            float top = -INFINITY, l = 0.0f;
+            for (int j = 0; j < mine; ++j) {
+                const int unit = w.halves ? 2 * j + s : j, key0 = (piece.k0 + unit) * MANY_KEYS;
+                if (!__all_sync(0xffffffffu, wait_or_abort(&s_bar[s], s_phase, abort_flag))) { ok = false; break; }
+                s_phase ^= 1;
+                after_sync();
+                const bool some_hidden = key0 + MANY_KEYS > limit_warp;
+                const int cols = limit - key0;               // columns below this are seen
+                if (warp_valid) {
+                    float big = -INFINITY;
+#pragma unroll 1
+                    for (int k = 0; k < MANY_KEYS; k += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(s_at + k, x);
+                        if (some_hidden) {
+#pragma unroll
+                            for (int q = 0; q < 32; ++q) if (k + q < cols) big = fmaxf(big, __uint_as_float(x[q]));
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 32; ++q) big = fmaxf(big, __uint_as_float(x[q]));
+                        }
+                    }
+                    big = valid ? big * c : -INFINITY;   // (what lies in other rows must not decide)
+                    if (__any_sync(0xffffffffu, big > top + 8.0f)) {     // (true too for the first)
+                        const float higher = fmaxf(top, big), f = top == -INFINITY ? 0.0f : ex2(top - higher);
+                        if (__any_sync(0xffffffffu, top != -INFINITY)) {
+                            // the products up to here are done: the score product that was waited for came after them
+#pragma unroll 1
+                            for (int k = 0; k < HD; k += 32) {
+                                uint32_t x[32];
+                                tmem_ld32(o_at + k, x);
+#pragma unroll
+                                for (int q = 0; q < 32; ++q) x[q] = __float_as_uint(__uint_as_float(x[q]) * f);
+                                tmem_st32(o_at + k, x);
+                            }
+                        }
+                        l *= f;
+                        top = higher;
+                    }
+                    const float b = top == -INFINITY ? 0.0f : top;
+#pragma unroll 1
+                    for (int k = 0; k < MANY_KEYS; k += 32) {
+                        uint32_t x[32], y[16];
+                        tmem_ld32(s_at + k, x);
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) {
+                            float e = ex2(fmaf(__uint_as_float(x[q]), c, -b));
+                            if (some_hidden) e = k + q < cols ? e : 0.0f;
+                            l += e;
+                            x[q] = __float_as_uint(e);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) y[q] = pack2<T>(__uint_as_float(x[2 * q]), __uint_as_float(x[2 * q + 1]));
+                        tmem_st16(s_at + k / 2, y);
+                    }
+                    tmem_wait_st();
+                }
+                if (key0 + MANY_KEYS > limit_all) {
+                    // Not all rows see all of these keys: zero weights must not meet infinities or NaN. Values behind the last seen key are made zero; of those
+                    // that some rows see, the ones that are not finite are added row by row and then made zero too.
+                    const uint32_t v_item = item + place_of_values(w.halves, piece.n, unit), v_at = ring + (v_item % m.slots) * SLOT;
+                    if (!__all_sync(0xffffffffu, wait_or_abort(&full_bar[v_item % m.slots], (v_item / m.slots) & 1, abort_flag))) { ok = false; break; }
+                    const bool both = !w.halves && unit < w.units[0];
+                    auto meet = [&]() {                      // of all threads that read this unit
+                        if (both) { mbar_arrive(&both_bar); ok = __all_sync(0xffffffffu, wait_or_abort(&both_bar, both_phase, abort_flag)); both_phase ^= 1; }
+                        else { mbar_arrive(&alone_bar[s]); ok = __all_sync(0xffffffffu, wait_or_abort(&alone_bar[s], alone_phase, abort_flag)); alone_phase ^= 1; }
+                    };
+                    const int there = seen - key0;           // a thread to a key
+                    const bool looks = !both || s == 0;
+                    uint32_t *found = special_sh[both ? 2 + both_phase : s];
+                    if (looks) {
+                        bool special = false;
+                        if (r < there && st.own) {
+#pragma unroll
+                            for (int ch = 0; ch < HD / 8; ++ch) special |= any_special<T>(lds_128(v_at + swizzled(r, ch)));
+                        }
+                        const uint32_t word = __ballot_sync(0xffffffffu, special);
+                        if (lane == 0) found[warp & 3] = word;
+                        if (r >= there) {
+#pragma unroll
+                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch));
+                        }
+                        async_proxy_fence();
+                    }
+                    meet();
+                    if (!ok) break;
+                    volatile uint32_t *marks = found;
+                    if (marks[0] | marks[1] | marks[2] | marks[3]) {     // the same for all who meet
+#pragma unroll 1
+                        for (int key = 0; key < MANY_KEYS; ++key)
+                            if (marks[key >> 5] >> (key & 31) & 1) add_key<T, HD>(s_at, o_at, v_at, key, key < cols);
+                        const bool clear = looks && (marks[r >> 5] >> (r & 31) & 1);
+                        meet();                              // nobody needs them any more
+                        if (!ok) break;
+                        if (clear) {
+#pragma unroll
+                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch));
+                        }
+                        async_proxy_fence();
+                        meet();
+                        if (!ok) break;
+                    }
+                }
+                before_sync();
+                mbar_arrive(&p_bar[s]);
+            }
+            if (!ok) break;
+
+            // ---- the piece's results ----
+            ok = __all_sync(0xffffffffu, wait_or_abort(&o_bar[s], turn & 1, abort_flag));
+            if (!ok) break;
+            after_sync();
+            const bool whole = piece.n == piece.ut && st.own && !w.halves && group_of(p, piece.e - p.n_groups) < 0;      // nothing to join with
+            const long long place = (line.tile[piece.e] + (long long)piece.h * piece.tiles + piece.t + blockIdx.x) * MANY_ROWS + s * HALF_ROWS + r;
+            if (warp_valid) {
+                const float inv = 1.0f / l;
+                uint4 *to = whole ? reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.d_out) + (long long)(row0 + i / p.G) * a.out_ld + (size_t)(piece.h * p.G + i % p.G) * HD)
+                                  : reinterpret_cast<uint4 *>(out.acc + place * HD);
+#pragma unroll 1
+                for (int k = 0; k < HD; k += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(o_at + k, x);
+                    if (!valid) continue;
+                    if (whole) {
+                        uint32_t y[16];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) y[q] = pack2<T>(__uint_as_float(x[2 * q]) * inv, __uint_as_float(x[2 * q + 1]) * inv);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) to[k / 8 + q] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) to[k / 4 + q] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+                    }
+                }
+                if (valid && !whole) out.top[place] = make_float2(top, l);
+            }
+            before_sync();
+            if (w.halves && s == 0) ok = __all_sync(0xffffffffu, wait_or_abort(&o_bar[1], turn & 1, abort_flag));       // the other stream reads this one's queries
+            ++turn;
+            item += 2 * piece.n;
+        }
+        if (!ok && lane == 0) give_up();
+    }
+
+    before_sync();
+    __syncthreads();
+    if (*abort_flag)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);     // copies in flight land before the memory is released
+    if (warp == 1) {
+        after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// pool [n_pages * n_kv][page][hd]; a box is 64 numbers of `box` tokens
+bool pool_map(CUtensorMap *map, const void *pool, const b200_paged_attn_args &a, int box)
+{
+    encode_fn_t enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.page, (cuuint64_t)a.n_pages * a.n_kv};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.hd * 2, (cuuint64_t)a.hd * 2 * a.page};
+    const cuuint32_t extent[3] = {64, (cuuint32_t)box, 1}, step[3] = {1, 1, 1};
+    return enc(map, a.wtype == B200_WT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(pool), dims, strides, extent, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st)
+{
+    constexpr size_t SLOT = BLOCK64 * (HD / 64);
+    const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), room = 227 * 1024 - 1024 - 1024;    // static memory, alignment
+    ManyArgs m;
+    m.slots = (int)((room - 2 * SLOT - plan) / SLOT);
+    if (m.slots > MOST_SLOTS) m.slots = MOST_SLOTS;
+    m.plan_off = (int)((2 + m.slots) * SLOT);
+    const size_t smem = m.plan_off + plan + 1024;
+    const int box = a.page < MANY_KEYS ? a.page : MANY_KEYS;
+    CUtensorMap mk, mv;
+    if (!pool_map(&mk, a.d_k_pool, a, box) || !pool_map(&mv, a.d_v_pool, a, box)) return B200_E_STATE;
+    cudaError_t e = cudaFuncSetAttribute(attn_many_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)out.workers);
+    cfg.blockDim = dim3(MANY_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attn_many_kernel<T, HD>, mk, mv, a, cut, out, m);
+    if (e != cudaSuccess) return (int)e;
+    ++g_b200_launches;
+    return 0;
+}
+
+}  // namespace
+
+int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st)
+{
+    if (a.wtype == B200_WT_F16) return a.hd == 64 ? launch<__half, 64>(a, cut, out, st) : launch<__half, 128>(a, cut, out, st);
+    return a.hd == 64 ? launch<__nv_bfloat16, 64>(a, cut, out, st) : launch<__nv_bfloat16, 128>(a, cut, out, st);
+}

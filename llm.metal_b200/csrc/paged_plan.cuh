@@ -8,17 +8,27 @@
 #include "stream_core.cuh"
 #include "../../include/llmb200_paged_kernels.h"
 
-namespace {
-
 // The sets that a kernel deals with: those of more than `lo` and at most `hi` query rows, in tiles of RT rows and units of KU keys.
-struct Cut { int rt, ku, lo, hi; };
+// A worker takes `least` units at least.
+struct Cut { int rt, ku, lo, hi, least; };
+
+// Where a cut's pieces lie in d_work: [slot][rt][hd] sums and [slot][rt] (largest score, sum), scores in units of log 2. A tile's piece of worker w is in
+// slot tile + w: the number of a piece never falls from one to the next on the line, and one of the two grows.
+struct Pieces { float *acc; float2 *top; long long workers; };
+
+namespace {
 
 // What a block knows of the step, in shared memory.
 struct Plan {
     int *row, *len, *group, *prefix;     // [n_req + 1], [n_req], [n_groups + 1], [n_groups]
+    char *lines;                         // room for the lines
+    int n_req, n_groups, n_kv, G;
+};
+// One cut's line.
+struct Line {
     long long *unit;                     // [sets + 1]: units before each set; groups' prefixes first, then requests
     int *tile;                           // [sets + 1]: (head, tile) pairs before each set
-    int n_req, n_groups, n_kv, G;
+    long long units, per;                // all units; those of a worker
 };
 
 __host__ __device__ inline size_t plan_bytes(int n_req, int n_groups, int cuts)
@@ -79,9 +89,8 @@ __device__ inline bool load_plan(const b200_paged_attn_args &a, Plan &p, char *m
 {
     const int sets = a.n_req + a.n_groups;
     p.n_req = a.n_req; p.n_groups = a.n_groups; p.n_kv = a.n_kv; p.G = a.n_q / a.n_kv;
-    p.unit = reinterpret_cast<long long *>(mem);
-    p.tile = reinterpret_cast<int *>(p.unit + (size_t)cuts * (sets + 1));
-    p.row = p.tile + (size_t)cuts * (sets + 2);
+    p.lines = mem;
+    p.row = reinterpret_cast<int *>(mem + (size_t)cuts * ((sets + 1) * 8 + (sets + 2) * 4));
     p.len = p.row + a.n_req + 1;
     p.group = p.len + a.n_req + 1;
     p.prefix = p.group + a.n_groups + 1;
@@ -109,20 +118,30 @@ __device__ inline bool load_plan(const b200_paged_attn_args &a, Plan &p, char *m
     return !bad;
 }
 
-// Lays the line of one cut. Returns its units. `red`: 32 long longs and 32 ints.
-__device__ inline long long lay_line(Plan &p, const Cut &c, long long *red, int *red_t)
+// Units of a worker: equal stretches, and none so short that joining costs more than it spreads.
+__device__ __forceinline__ long long stretch(long long units, long long workers, int least)
+{
+    const long long per = (units + workers - 1) / workers;
+    return per < least ? least : per;
+}
+
+// Lays the line of a cut that `workers` share, in the k-th room for one. `red`: 32 long longs and 32 ints.
+__device__ inline Line lay_line(const Plan &p, const Cut &c, int k, long long workers, long long *red, int *red_t)
 {
     const int sets = p.n_req + p.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    Line line;
+    line.unit = reinterpret_cast<long long *>(p.lines + (size_t)k * ((sets + 1) * 8));
+    line.tile = reinterpret_cast<int *>(reinterpret_cast<char *>(p.row) - (size_t)(k + 1) * (sets + 2) * 4);
     const int each = (sets + blockDim.x - 1) / blockDim.x, e0 = min(sets, (int)threadIdx.x * each), e1 = min(sets, e0 + each);
     long long u = 0;
     int t = 0;
     for (int e = e0; e < e1; ++e) {
         const Set s = set_at(p, e);
         long long n = 0;
-        int k = 0;
-        if (in_cut(s, c)) { k = tiles_of(s, c); n = units_before(p, s, c, k) * p.n_kv; k *= p.n_kv; }
-        p.unit[e] = n; p.tile[e] = k;                        // summed up below, by the same thread
-        u += n; t += k;
+        int m = 0;
+        if (in_cut(s, c)) { m = tiles_of(s, c); n = units_before(p, s, c, m) * p.n_kv; m *= p.n_kv; }
+        line.unit[e] = n; line.tile[e] = m;                  // summed up below, by the same thread
+        u += n; t += m;
     }
     long long iu = u;
     int it = t;
@@ -143,14 +162,64 @@ __device__ inline long long lay_line(Plan &p, const Cut &c, long long *red, int 
         all += red[w]; all_t += red_t[w];
     }
     for (int e = e0; e < e1; ++e) {
-        const long long n = p.unit[e];
-        const int k = p.tile[e];
-        p.unit[e] = iu; p.tile[e] = it;
-        iu += n; it += k;
+        const long long n = line.unit[e];
+        const int m = line.tile[e];
+        line.unit[e] = iu; line.tile[e] = it;
+        iu += n; it += m;
     }
-    if (threadIdx.x == 0) { p.unit[sets] = all; p.tile[sets] = all_t; }
+    if (threadIdx.x == 0) { line.unit[sets] = all; line.tile[sets] = all_t; }
     __syncthreads();
-    return all;
+    line.units = all;
+    line.per = stretch(all, workers, c.least);
+    return line;
+}
+
+// One worker's way along a line: the pieces of its stretch, one after the other.
+struct Piece {
+    int e, h, t, tiles;                  // set, key / value head, tile, tiles of a head
+    int k0, n, ut;                       // its units k0 .. k0 + n - 1 of the tile's ut
+    Set s;
+};
+struct Walk {
+    long long at, end;
+    int e;
+    __device__ __forceinline__ Walk(const Plan &p, const Line &line, long long worker)
+    {
+        at = worker * line.per;
+        end = min(line.units, at + line.per);
+        e = at < end ? last_at(line.unit, p.n_req + p.n_groups, at) : 0;
+    }
+    __device__ __forceinline__ bool next(const Plan &p, const Line &line, const Cut &c, Piece &q)
+    {
+        if (at >= end) return false;
+        while (line.unit[e + 1] <= at) ++e;
+        q.e = e;
+        q.s = set_at(p, e);
+        q.tiles = tiles_of(q.s, c);
+        const long long head_units = (line.unit[e + 1] - line.unit[e]) / p.n_kv;
+        q.h = (int)((at - line.unit[e]) / head_units);
+        long long rest = at - line.unit[e] - q.h * head_units;
+        q.t = 0;
+        q.ut = units_of(p, q.s, c, 0);
+        while (rest >= q.ut) { rest -= q.ut; q.ut = units_of(p, q.s, c, ++q.t); }
+        q.k0 = (int)rest;
+        q.n = (int)min((long long)(q.ut - q.k0), end - at);
+        at += q.n;
+        return true;
+    }
+};
+
+// Whether the rows of a request have keys in a prefix: its group, or -1.
+__device__ __forceinline__ int group_of(const Plan &p, int r)
+{
+    if (!p.n_groups || r < p.group[0] || r >= p.group[p.n_groups]) return -1;
+    const int g = last_at(p.group, p.n_groups, r);
+    return p.prefix[g] > 0 ? g : -1;
+}
+__device__ __forceinline__ int first_row(const Plan &p, const Piece &q) { return q.s.own ? p.row[q.e - p.n_groups] : p.row[p.group[q.e]]; }
+__device__ __forceinline__ const int *pages_of(const b200_paged_attn_args &a, const Piece &q)
+{
+    return q.s.own ? a.d_table + (size_t)(q.e - a.n_groups) * a.table_ld : a.d_prefix_table + (size_t)q.e * a.prefix_ld;
 }
 
 }  // namespace
