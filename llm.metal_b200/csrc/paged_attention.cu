@@ -11,8 +11,8 @@
 
 namespace {
 
-constexpr int FEW_ROWS = 16, FEW_KEYS = 16, FEW_WARPS = 4, FEW_STAGES = 3, FEW_LEAST = 4;
-constexpr int JOIN_WARPS = 8;
+constexpr int FEW_ROWS = 16, FEW_KEYS = 16, FEW_WARPS = 4, FEW_STAGES = 3, FEW_LEAST = 4, FEW_GAP = 1;
+constexpr int JOIN_WARPS = 8, JOIN_BLOCKS = 4;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on)
 {
@@ -39,7 +39,7 @@ template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const
 }
 template <typename T, int HD>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
-attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces out, int beside)
+attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, const Pieces out, int big, int beside)
 {
     constexpr int CH = HD / 8;                               // 16-byte chunks of a key
     constexpr int HALF_STAGE = FEW_KEYS * HD * 2, STAGE = 2 * HALF_STAGE;
@@ -52,8 +52,9 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
     // is there. Its results are waited for at the end, for the join's sake, whose own wait covers this grid alone.
     if (!beside) pdl_wait();
     Plan p;
-    if (!load_plan(a, p, smem + FEW_WARPS * FEW_STAGES * STAGE, 1)) { pdl_wait(); return; }
-    const Line line = lay_line(p, cut, 0, out.workers, red, red_t);
+    if (!load_plan(a, p, smem + FEW_WARPS * FEW_STAGES * STAGE, 1, big, red_t)) { pdl_wait(); return; }
+    Line line;
+    if (!lay_line(a, p, cut, 0, out.workers, line, red, red_t)) { pdl_wait(); return; }
     const int worker = blockIdx.x * FEW_WARPS + warp;
     const uint32_t ring = smem_u32(smem) + warp * FEW_STAGES * STAGE;
     const uint16_t *kp = static_cast<const uint16_t *>(a.d_k_pool), *vp = static_cast<const uint16_t *>(a.d_v_pool);
@@ -67,17 +68,18 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
         // ---- query rows t * 16 .. of head h, units k0 .. k0 + n - 1 ----
         const Set &s = piece.s;
         const int e = piece.e, h = piece.h, t = piece.t, k0 = piece.k0, n = piece.n;
-        const int row0 = first_row(p, piece), i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
+        const int i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
         const int seen = seen_by(p, s, cut, t), seen_first = s.own ? s.keys - s.rows + i0 / p.G + 1 : s.keys;
-        const int *table = pages_of(a, piece);
-        int limit[2];
+        const int *table = part_at(a, p, cut, piece, 0).table;
+        int limit[2], row_of[2];
         uint32_t q[CH / 2][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int i = i0 + g + 8 * half;
             const bool on = g + 8 * half < valid;
             limit[half] = !on ? 0 : s.own ? s.keys - s.rows + i / p.G + 1 : s.keys;
-            const uint16_t *src = static_cast<const uint16_t *>(a.d_q) + (long long)(row0 + (on ? i / p.G : 0)) * a.q_ld + (size_t)(h * p.G + (on ? i % p.G : 0)) * HD + 2 * cq;
+            row_of[half] = row_at(p, e, on ? i / p.G : 0);
+            const uint16_t *src = static_cast<const uint16_t *>(a.d_q) + (long long)row_of[half] * a.q_ld + (size_t)(h * p.G + (on ? i % p.G : 0)) * HD + 2 * cq;
 #pragma unroll
             for (int ks = 0; ks < CH / 2; ++ks) {
                 q[ks][half] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * ks) : 0u;
@@ -207,7 +209,7 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
-        const bool whole = n == piece.ut && s.own && group_of(p, e - p.n_groups) < 0;          // nothing to join with
+        const bool whole = n == piece.ut && alone(p, piece);          // nothing to join with
         const long long slot = line.tile[e] + (long long)h * piece.tiles + t + worker;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -215,7 +217,7 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
             if (k >= valid) continue;
             if (whole) {
                 const float inv = 1.0f / l[r];
-                uint16_t *to = static_cast<uint16_t *>(a.d_out) + (long long)(row0 + i / p.G) * a.out_ld + (size_t)(h * p.G + i % p.G) * HD + 2 * cq;
+                uint16_t *to = static_cast<uint16_t *>(a.d_out) + (long long)row_of[r] * a.out_ld + (size_t)(h * p.G + i % p.G) * HD + 2 * cq;
 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch) *reinterpret_cast<uint32_t *>(to + 8 * ch) = pack2<T>(o[ch][2 * r] * inv, o[ch][2 * r + 1] * inv);
             } else {
@@ -231,7 +233,7 @@ attn_few_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut, c
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut0, const Pieces in0, const Cut cut1, const Pieces in1)
+attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut0, const Pieces in0, const Cut cut1, const Pieces in1, int big)
 {
     constexpr int N = HD / 32;                               // numbers of a lane, next to one another
     extern __shared__ __align__(128) char smem[];
@@ -241,62 +243,66 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const Cut cut0,
     pdl_launch_dependents();
     pdl_wait();
     Plan p;
-    if (!load_plan(a, p, smem, 2)) return;
-    const Line few = lay_line(p, cut0, 0, in0.workers, red, red_t), many = lay_line(p, cut1, 1, in1.workers, red, red_t);
-    const long long at = (long long)blockIdx.x * JOIN_WARPS + warp;
-    const int row = (int)(at / a.n_q), head = (int)(at % a.n_q);
-    if (row >= p.row[p.n_req]) return;
-    const int r = last_at(p.row, p.n_req, row), h = head / p.G, group = group_of(p, r);
-    // the row's pieces of the prefix and of the own tokens: where the first one lies, how many, how far apart
-    const float *acc[2] = {};
-    const float2 *tops[2] = {};
-    int count[2] = {0, 0}, step[2] = {0, 0};
-    bool cut_up = false;
+    if (!load_plan(a, p, smem, 2, big, red_t)) return;
+    Line few, many;
+    if (!lay_line(a, p, cut0, 0, in0.workers, few, red, red_t) || !lay_line(a, p, cut1, 1, in1.workers, many, red, red_t)) return;
+    const long long all = (long long)p.row[p.n_req] * a.n_q;
+    for (long long at = (long long)blockIdx.x * JOIN_WARPS + warp; at < all; at += (long long)gridDim.x * JOIN_WARPS) {
+        const int row = (int)(at / a.n_q), head = (int)(at % a.n_q);
+        const int r = last_at(p.row, p.n_req, row), h = head / p.G;
+        int group = group_of(p, r);
+        if (is_big(p, r, group)) group = -1;                 // one set
+        // the row's pieces of the prefix and of the own tokens: where the first one lies, how many, how far apart
+        const float *acc[2] = {};
+        const float2 *tops[2] = {};
+        int count[2] = {0, 0}, step[2] = {0, 0};
+        bool cut_up = false;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int e = k == 0 ? group : p.n_groups + r;
-        if (e < 0) continue;
-        const Set s = set_at(p, e);
-        const bool is_few = in_cut(s, cut0);
-        const Cut &cut = is_few ? cut0 : cut1;
-        const Line &line = is_few ? few : many;
-        const Pieces &in = is_few ? in0 : in1;
-        const int i = (row - (s.own ? p.row[r] : p.row[p.group[e]])) * p.G + head % p.G, t = i / cut.rt, tiles = tiles_of(s, cut);
-        const long long head_units = (line.unit[e + 1] - line.unit[e]) / p.n_kv;
-        const long long b = line.unit[e] + h * head_units + units_before(p, s, cut, t), w0 = b / line.per, w1 = (b + units_of(p, s, cut, t) - 1) / line.per;
-        // a tile of 128 rows at most, in places for 256: two pieces in each, of every other unit
-        const bool halves = !is_few && s.nr - t * MANY_ROWS <= MANY_ROWS / 2;
-        const long long place = (line.tile[e] + (long long)h * tiles + t + w0) * cut.rt + i % cut.rt;
-        acc[k] = in.acc + place * HD;
-        tops[k] = in.top + place;
-        step[k] = halves ? cut.rt / 2 : cut.rt;
-        count[k] = (int)(w1 - w0 + 1) * (halves ? 2 : 1);
-        cut_up |= w1 > w0 || halves;
-    }
-    const int n = count[0] + count[1];
-    if (group < 0 && !cut_up) return;                        // stored where it was formed
-    auto top_of = [&](int j) { return j < count[0] ? tops[0][(long long)j * step[0]] : tops[1][(long long)(j - count[0]) * step[1]]; };
-    auto acc_of = [&](int j) { return j < count[0] ? acc[0] + (long long)j * step[0] * HD : acc[1] + (long long)(j - count[0]) * step[1] * HD; };
-    float top = -INFINITY;
-    for (int j = lane; j < n; j += 32) top = fmaxf(top, top_of(j).x);
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, o[N];
+        for (int k = 0; k < 2; ++k) {
+            const int e = k == 0 ? group : p.n_groups + r;
+            if (e < 0) continue;
+            const Set s = set_at(p, e);
+            const bool is_few = in_cut(s, cut0);
+            const Cut &cut = is_few ? cut0 : cut1;
+            const Line &line = is_few ? few : many;
+            const Pieces &in = is_few ? in0 : in1;
+            const int i = (row - p.row[r] + (s.own ? 0 : p.small[r] - p.small[p.group[e]])) * p.G + head % p.G, t = i / cut.rt, tiles = tiles_of(s, cut);
+            const int per_head = (line.unit[e + 1] - line.unit[e]) / p.n_kv;
+            const int b = line.unit[e] + h * per_head + (int)line_before(p, s, cut, t) + cut.gap, w0 = b / line.per, w1 = (b + units_of(p, s, cut, t) - 1) / line.per;
+            // a tile of 128 rows at most, in places for 256: two pieces in each, of every other unit
+            const bool halves = !is_few && s.nr - t * MANY_ROWS <= MANY_ROWS / 2;
+            const long long place = (long long)(line.tile[e] + h * tiles + t + w0) * cut.rt + i % cut.rt;
+            acc[k] = in.acc + place * HD;
+            tops[k] = in.top + place;
+            step[k] = halves ? cut.rt / 2 : cut.rt;
+            count[k] = (w1 - w0 + 1) * (halves ? 2 : 1);
+            cut_up |= w1 > w0 || halves;
+        }
+        const int n = count[0] + count[1];
+        if (group < 0 && !cut_up) continue;                      // stored where it was formed
+        auto top_of = [&](int j) { return j < count[0] ? tops[0][(long long)j * step[0]] : tops[1][(long long)(j - count[0]) * step[1]]; };
+        auto acc_of = [&](int j) { return j < count[0] ? acc[0] + (long long)j * step[0] * HD : acc[1] + (long long)(j - count[0]) * step[1] * HD; };
+        float top = -INFINITY;
+        for (int j = lane; j < n; j += 32) top = fmaxf(top, top_of(j).x);
+        top = warp_max(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f, o[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+        for (int i = 0; i < N; ++i) o[i] = 0.0f;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-        const float2 ml = top_of(j);
-        const float f = ex2(ml.x - base);
-        const float *v = acc_of(j) + lane * N;
-        l = fmaf(ml.y, f, l);
+        for (int j = 0; j < n; ++j) {
+            const float2 ml = top_of(j);
+            const float f = ex2(ml.x - base);
+            const float *v = acc_of(j) + lane * N;
+            l = fmaf(ml.y, f, l);
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(v[i], f, o[i]);
+            for (int i = 0; i < N; ++i) o[i] = fmaf(v[i], f, o[i]);
+        }
+        const float inv = 1.0f / l;
+        uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)head * HD + lane * N);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) to[i / 2] = pack2<T>(o[i] * inv, o[i + 1] * inv);
     }
-    const float inv = 1.0f / l;
-    uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)head * HD + lane * N);
-#pragma unroll
-    for (int i = 0; i < N; i += 2) to[i / 2] = pack2<T>(o[i] * inv, o[i + 1] * inv);
 }
 
 int sm_count()
@@ -321,14 +327,14 @@ int check_sizes(const b200_paged_attn_args &a)
 // Sets of more query rows than this go to attn_many_kernel, where hd is one of its own.
 constexpr int FEW_MOST = 16;
 
-struct Layout { long long few_workers, many_workers; size_t few_acc, few_top, many_acc, many_top, bytes; };
+struct Layout { int few_workers, many_workers; size_t few_acc, few_top, many_acc, many_top, bytes; };
 
 Layout layout_of(const b200_paged_attn_args &a)
 {
     const long long G = a.n_q / a.n_kv, all = a.max_rows * G * (a.n_groups ? 2 : 1);         // query rows of all sets
     const long long sets = (a.n_req < a.max_rows ? a.n_req : a.max_rows) + (a.n_groups < a.max_rows ? a.n_groups : a.max_rows);
     Layout L = {};
-    L.few_workers = 2LL * sm_count() * FEW_WARPS;
+    L.few_workers = 2 * sm_count() * FEW_WARPS;
     L.many_workers = a.hd <= 128 && all > FEW_MOST ? sm_count() : 0;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
     const long long few_most = L.many_workers ? FEW_MOST : all;
@@ -352,10 +358,11 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     char *work = static_cast<char *>(a.d_work);
     const Pieces few = {reinterpret_cast<float *>(work + L.few_acc), reinterpret_cast<float2 *>(work + L.few_top), L.few_workers};
     const Pieces many = {reinterpret_cast<float *>(work + L.many_acc), reinterpret_cast<float2 *>(work + L.many_top), L.many_workers};
-    const Cut few_cut = {FEW_ROWS, FEW_KEYS, 0, L.many_workers ? FEW_MOST : INT_MAX, FEW_LEAST};
-    const Cut many_cut = {MANY_ROWS, MANY_KEYS, L.many_workers ? FEW_MOST : INT_MAX, INT_MAX, MANY_LEAST};
+    const Cut few_cut = {FEW_ROWS, FEW_KEYS, 0, L.many_workers ? FEW_MOST : INT_MAX, FEW_LEAST, FEW_GAP};
+    const Cut many_cut = {MANY_ROWS, MANY_KEYS, L.many_workers ? FEW_MOST : INT_MAX, INT_MAX, MANY_LEAST, MANY_GAP};
+    const int big = L.many_workers ? BIG_ROWS : INT_MAX;
     if (L.many_workers)
-        if (const int rc = attn_many_launch(a, many_cut, many, st)) return rc;
+        if (const int rc = attn_many_launch(a, many_cut, many, big, st)) return rc;
     const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), smem = (size_t)FEW_WARPS * FEW_STAGES * 2 * FEW_KEYS * HD * 2 + plan;
     cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
@@ -369,13 +376,13 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0 || L.many_workers;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD>, a, few_cut, few, (int)(L.many_workers != 0));
+    e = cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD>, a, few_cut, few, big, (int)(L.many_workers != 0));
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
     const size_t both = plan_bytes(a.n_req, a.n_groups, 2);
     if (both > 48 * 1024 && (e = cudaFuncSetAttribute(attn_join_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)both)) != cudaSuccess) return (int)e;
-    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS)), dim3(JOIN_WARPS * 32), both, st, a, few_cut, few,
-                       many_cut, many);
+    const long long blocks = ((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS, most = JOIN_BLOCKS * sm_count();
+    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(JOIN_WARPS * 32), both, st, a, few_cut, few, many_cut, many, big);
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
     return (int)cudaGetLastError();

@@ -44,9 +44,10 @@ template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v
     return any;
 }
 
-constexpr int MANY_ROWS = 256, MANY_KEYS = 128, MANY_LEAST = 2;
+// BIG_ROWS: a request of that many query rows fills a stream of attn_many_kernel by itself.
+constexpr int MANY_ROWS = 256, MANY_KEYS = 128, MANY_LEAST = 2, MANY_GAP = 3, BIG_ROWS = 128;
 
 }  // namespace
 
 // attn_many_kernel (paged_attention_many.cu): the sets of more than `lo` query rows, hd 64 or 128. One block to an SM.
-int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st);
+int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st);

@@ -50,6 +50,36 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) { tmem_st16(taddr, r); tmem_st16(taddr + 16, r + 16); }
+// 128 columns of the lanes' rows
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
+        "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+        "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+        "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr)
 {
@@ -64,6 +94,21 @@ __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.
 
 __device__ __forceinline__ uint32_t swizzled(int row, int ch) { return (ch >> 3) * BLOCK64 + row * 128 + (((ch & 7) ^ (row & 7)) * 16); }     // chunk ch of a row
 __device__ __forceinline__ void zero16(uint32_t at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory"); }
+
+// The rows' results times f: by the whole warp. Eight columns at a time: a row of scores is held meanwhile.
+template <int HD> __device__ __forceinline__ void scale_rows(uint32_t o_at, float f)
+{
+#pragma unroll 1
+    for (int k = 0; k < HD; k += 8) {
+        uint32_t x[8];
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]) : "r"(o_at + k) : "memory");
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = __float_as_uint(__uint_as_float(x[q]) * f);
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"r"(o_at + k), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+    }
+}
 
 // The rows' results plus weight times value of one key, for rows that see it: by the whole warp.
 template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at, uint32_t o_at, uint32_t v_at, int key, bool sees)
@@ -97,14 +142,14 @@ struct Streams {
     bool halves;                         // one tile of rows, every other unit to a stream
     int units[2];
 };
-__device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q)
+__device__ __forceinline__ Streams streams_of(const Plan &p, const Cut &c, const Piece &q)
 {
     Streams w;
     const int valid = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS);
     w.halves = valid <= HALF_ROWS;
     if (w.halves) { w.units[0] = (q.n + 1) / 2; w.units[1] = q.n / 2; return w; }
     const int seen = q.s.own ? q.s.keys - q.s.rows + (q.t * MANY_ROWS + HALF_ROWS - 1) / p.G + 1 : q.s.keys;
-    w.units[0] = max(0, min(q.n, (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
+    w.units[0] = max(0, min(q.n, units_before_own(q.s, c) + (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
     w.units[1] = q.n;
     return w;
 }
@@ -114,7 +159,7 @@ __device__ __forceinline__ int place_of_values(bool halves, int n, int j) { retu
 template <typename T, int HD>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ b200_paged_attn_args a, const Cut cut,
-                 const Pieces out, const ManyArgs m)
+                 const Pieces out, const ManyArgs m, int big)
 {
     constexpr int NB = HD / 64;
     constexpr uint32_t SLOT = BLOCK64 * NB, Q_TILE = BLOCK64 * NB;
@@ -125,6 +170,8 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2], p_bar[2], o_bar[2], alone_bar[2], both_bar;
     __shared__ long long red[32];
     __shared__ int red_t[32];
+    __shared__ Plan plan_sh;
+    __shared__ Line line_sh;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_sh;
     __shared__ uint32_t special_sh[4][4];
@@ -153,129 +200,20 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t tmem = tmem_sh;
     pdl_wait();
     pdl_launch_dependents();                                 // after the wait: attn_few_kernel starts on this and waits for nothing else
-    Plan p;
-    const bool fits = load_plan(a, p, base + m.plan_off, 1);
-    Line line = {};
-    if (fits) line = lay_line(p, cut, 0, out.workers, red, red_t);
-    Walk walk(p, line, fits ? blockIdx.x : 0);
-    Piece piece;
+    {
+        Plan plan;
+        Line laid;
+        if (!load_plan(a, plan, base + m.plan_off, 1, big, red_t) || !lay_line(a, plan, cut, 0, out.workers, laid, red, red_t)) laid.units = laid.per = 0;
+        if (threadIdx.x == 0) { plan_sh = plan; line_sh = laid; }
+        __syncthreads();
+    }
+    const Plan &p = plan_sh;                                 // in shared memory: registers are for the scores
+    const Line &line = line_sh;
     auto give_up = [&]() { if (!*abort_flag) { *abort_flag = 1; if (a.d_status) atomicOr(a.d_status, B200_PAGED_TIMED_OUT); } };
 
-    if (warp == 0) {
-        // ---- pages into the ring ----
-        const int box = min(a.page, MANY_KEYS), page_shift = 31 - __clz(a.page), boxes = MANY_KEYS / box;
-        asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
-        uint32_t item = 0;
-        bool outside = false, ok = true;
-        while (ok && walk.next(p, line, cut, piece)) {
-            const Streams w = streams_of(p, piece);
-            const int *table = pages_of(a, piece);
-            const int seen = seen_by(p, piece.s, cut, piece.t), n = piece.n;
-            auto load = [&](int unit, bool values) {         // by the whole warp
-                const int slot = item % m.slots;
-                const uint32_t phase = (item / m.slots) & 1;
-                ++item;
-                const int key0 = (piece.k0 + unit) * MANY_KEYS, there = min(boxes, (seen - key0 + box - 1) / box);
-                const int mine = lane / NB, part = lane % NB, key = key0 + mine * box;
-                int id = mine < there ? __ldg(table + (key >> page_shift)) : 0;
-                if (id < 0 || id >= a.n_pages) { outside = true; id = -1; }
-                if (!__all_sync(0xffffffffu, wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag))) { ok = false; return; }
-                if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)there * box * 128 * NB);
-                __syncwarp();
-                if (mine < there)                            // an id of -1 is outside the map and reads as zeros
-                    tma_load_3d(ring + slot * SLOT + part * BLOCK64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
-                                id < 0 ? -1 : id * a.n_kv + piece.h, &full_bar[slot]);
-            };
-            if (w.halves) {
-                load(0, false);
-                if (ok && n > 1) load(1, false);
-                for (int j = 0; j < n && ok; ++j) {
-                    load(j, true);
-                    if (ok && j + 2 < n) load(j + 2, false);
-                }
-            } else {
-                for (int j = 0; j < n && ok; ++j) {
-                    load(j, false);
-                    if (ok) load(j, true);
-                }
-            }
-        }
-        if (!ok) give_up();
-        if (outside && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
-    } else if (warp == 1) {
-        // ---- the products ----
-        if (lane == 0) {
-            uint32_t item = 0, turn = 0, p_phase[2] = {0, 0};
-            bool ok = true;
-            auto full = [&](uint32_t i) {
-                if (ok && !wait_or_abort(&full_bar[i % m.slots], (i / m.slots) & 1, abort_flag)) ok = false;
-                after_sync();
-            };
-            auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % m.slots]); };
-            while (ok && walk.next(p, line, cut, piece)) {
-                const Streams w = streams_of(p, piece);
-                const int n = piece.n;
-                for (int s = 0; s < 2 && ok; ++s) ok = wait_or_abort(&q_bar[s], turn & 1, abort_flag);
-                ++turn;
-                if (!ok) break;
-                after_sync();
-                auto scores = [&](int s, uint32_t i) {
-                    const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % m.slots) * SLOT;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint64_t qd = smem_desc_sw128(q + b * BLOCK64), kd = smem_desc_sw128(k + b * BLOCK64);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) umma_f16(tmem + S_COL + s * 128, qd + 2 * j, kd + 2 * j, IDESC_S, (b | j) != 0);
-                    }
-                    umma_commit(&s_bar[s]);
-                };
-                auto sums = [&](int s, uint32_t i) {
-                    if (!wait_or_abort(&p_bar[s], p_phase[s], abort_flag)) { ok = false; return; }
-                    p_phase[s] ^= 1;
-                    after_sync();
-                    const uint64_t vd = smem_desc_rows(ring + (i % m.slots) * SLOT, BLOCK64);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) umma_from_tmem(tmem + O_COL + s * 128, tmem + S_COL + s * 128 + 8 * j, vd + 128 * j, IDESC_O);
-                };
-                if (w.halves) {
-                    full(item);
-                    if (!ok) break;
-                    scores(0, item); release(item);
-                    if (n > 1) { full(item + 1); if (!ok) break; scores(1, item + 1); release(item + 1); }
-                    else umma_commit(&o_bar[1]);
-                    for (int j = 0; j < n && ok; ++j) {
-                        const uint32_t v = item + place_of_values(true, n, j);
-                        full(v);
-                        if (ok) sums(j & 1, v);
-                        if (!ok) break;
-                        release(v);
-                        if (j + 2 < n) { full(v + 1); if (!ok) break; scores(j & 1, v + 1); release(v + 1); }
-                        else umma_commit(&o_bar[j & 1]);
-                    }
-                } else {
-                    full(item);
-                    if (!ok) break;
-                    if (w.units[0] > 0) scores(0, item); else umma_commit(&o_bar[0]);
-                    scores(1, item); release(item);
-                    for (int j = 0; j < n && ok; ++j) {
-                        const uint32_t v = item + 2 * j + 1;
-                        full(v);
-                        if (ok && j < w.units[0]) {
-                            sums(0, v);
-                            if (!ok) break;
-                            if (j + 1 < w.units[0]) { full(v + 1); if (!ok) break; scores(0, v + 1); } else umma_commit(&o_bar[0]);
-                        }
-                        if (ok) sums(1, v);
-                        if (!ok) break;
-                        release(v);
-                        if (j + 1 < n) { full(v + 1); if (!ok) break; scores(1, v + 1); release(v + 1); } else umma_commit(&o_bar[1]);
-                    }
-                }
-                item += 2 * n;
-            }
-            if (!ok) give_up();
-        }
-    } else if (warp >= 4) {
+    // Registers: 168 a thread at the launch, 384 threads; 72 for four warps and 216 for the eight with a row of scores a thread are as many.
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- a stream's rows ----
         const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;       // stream, row of its tile = lane of tensor memory
         const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), s_at = tm + S_COL + s * 128, o_at = tm + O_COL + s * 128;
@@ -283,25 +221,29 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         uint32_t turn = 0, item = 0, s_phase = 0, alone_phase = 0, both_phase = 0;
         bool ok = true;
+        Walk walk(p, line, blockIdx.x);
+        Piece piece;
         while (ok && walk.next(p, line, cut, piece)) {
-            const Streams w = streams_of(p, piece);
+            const Streams w = streams_of(p, cut, piece);
             const Set &st = piece.s;
-            const int i0 = piece.t * MANY_ROWS, i = i0 + (w.halves ? 0 : s * HALF_ROWS) + r, row0 = first_row(p, piece);
-            const bool valid = i < st.nr;
-            const int seen = seen_by(p, st, cut, piece.t), mine = w.units[s];
-            // keys that this row sees, that the first row of the whole tile sees (all rows see), and the first one of this warp
-            const int limit = st.own ? st.keys - st.rows + min(i, st.nr - 1) / p.G + 1 : st.keys;
-            const int limit_all = st.own ? st.keys - st.rows + i0 / p.G + 1 : st.keys, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
-            const bool warp_valid = __any_sync(0xffffffffu, valid);
-            if (valid && !(w.halves && s == 1)) {
-                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.d_q) + (long long)(row0 + i / p.G) * a.q_ld + (size_t)(piece.h * p.G + i % p.G) * HD);
-                const uint32_t dst = q_tiles + s * Q_TILE;
+            const int i0 = piece.t * MANY_ROWS, i = i0 + (w.halves ? 0 : s * HALF_ROWS) + r, mine = w.units[s];
+            const bool valid = i < st.nr, warp_valid = __any_sync(0xffffffffu, valid);
+            const int row = row_at(p, piece.e, min(i, st.nr - 1) / p.G);
+            const size_t column = (size_t)(piece.h * p.G + min(i, st.nr - 1) % p.G) * HD;
+            // a warp's rows, HD / 8 lanes to each so that whole lines are read; all loads before the first store
+            constexpr int CH = HD / 8, RL = 32 / CH;         // 16-byte chunks of a row, rows of a load
+            const long long q_off = (long long)row * a.q_ld + column;
+            if (warp_valid && !(w.halves && s == 1)) {
+                uint4 v[32 / RL];
 #pragma unroll
-                for (int ch = 0; ch < HD / 8; ++ch) {
-                    const uint4 v = src[ch];
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + swizzled(r, ch)), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip),
-                                 "r"(v.w ^ flip) : "memory");
+                for (int k = 0; k < 32 / RL; ++k) {
+                    const long long off = __shfl_sync(0xffffffffu, q_off, k * RL + lane / CH);
+                    v[k] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.d_q) + off + (lane % CH) * 8);
                 }
+#pragma unroll
+                for (int k = 0; k < 32 / RL; ++k)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_tiles + s * Q_TILE + swizzled((warp & 3) * 32 + k * RL + lane / CH, lane % CH)),
+                                 "r"(v[k].x ^ flip), "r"(v[k].y ^ flip), "r"(v[k].z ^ flip), "r"(v[k].w ^ flip) : "memory");
             }
             async_proxy_fence();
             {
@@ -314,59 +256,49 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             mbar_arrive(&q_bar[s]);
             float top = -INFINITY, l = 0.0f;
             for (int j = 0; j < mine; ++j) {
-                const int unit = w.halves ? 2 * j + s : j, key0 = (piece.k0 + unit) * MANY_KEYS;
+                const int unit = w.halves ? 2 * j + s : j;
+                const Part u = part_at(a, p, cut, piece, unit);
+                // keys that this row sees, that the first row of this warp sees, that the first row of the whole tile sees (all rows see)
+                const int key0 = u.key0, limit = u.own ? st.keys - st.rows + min(i, st.nr - 1) / p.G + 1 : u.seen, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
+                const int limit_all = u.own ? st.keys - st.rows + i0 / p.G + 1 : u.seen;
                 if (!__all_sync(0xffffffffu, wait_or_abort(&s_bar[s], s_phase, abort_flag))) { ok = false; break; }
                 s_phase ^= 1;
                 after_sync();
                 const bool some_hidden = key0 + MANY_KEYS > limit_warp;
                 const int cols = limit - key0;               // columns below this are seen
                 if (warp_valid) {
-                    float big = -INFINITY;
-#pragma unroll 1
-                    for (int k = 0; k < MANY_KEYS; k += 32) {
-                        uint32_t x[32];
-                        tmem_ld32(s_at + k, x);
-                        if (some_hidden) {
+                    uint32_t x[128];
+                    tmem_ld128(s_at, x);
+                    if (some_hidden) {
 #pragma unroll
-                            for (int q = 0; q < 32; ++q) if (k + q < cols) big = fmaxf(big, __uint_as_float(x[q]));
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 32; ++q) big = fmaxf(big, __uint_as_float(x[q]));
-                        }
+                        for (int q = 0; q < 128; ++q) x[q] = q < cols ? x[q] : 0xff800000u;
                     }
-                    big = valid ? big * c : -INFINITY;   // (what lies in other rows must not decide)
+                    float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int q = 0; q < 128; ++q) big4[q & 3] = fmaxf(big4[q & 3], __uint_as_float(x[q]));
+                    const float big = valid ? fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3])) * c : -INFINITY;   // (what lies in other rows must not decide)
                     if (__any_sync(0xffffffffu, big > top + 8.0f)) {     // (true too for the first)
                         const float higher = fmaxf(top, big), f = top == -INFINITY ? 0.0f : ex2(top - higher);
-                        if (__any_sync(0xffffffffu, top != -INFINITY)) {
-                            // the products up to here are done: the score product that was waited for came after them
-#pragma unroll 1
-                            for (int k = 0; k < HD; k += 32) {
-                                uint32_t x[32];
-                                tmem_ld32(o_at + k, x);
-#pragma unroll
-                                for (int q = 0; q < 32; ++q) x[q] = __float_as_uint(__uint_as_float(x[q]) * f);
-                                tmem_st32(o_at + k, x);
-                            }
-                        }
+                        // the products up to here are done: the score product that was waited for came after them
+                        if (__any_sync(0xffffffffu, top != -INFINITY)) scale_rows<HD>(o_at, f);
                         l *= f;
                         top = higher;
                     }
-                    const float b = top == -INFINITY ? 0.0f : top;
-#pragma unroll 1
+                    const float b = top == -INFINITY ? 0.0f : -top;
+                    float2 sum[2] = {};
+#pragma unroll
                     for (int k = 0; k < MANY_KEYS; k += 32) {
-                        uint32_t x[32], y[16];
-                        tmem_ld32(s_at + k, x);
+                        uint32_t y[16];
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) {
-                            float e = ex2(fmaf(__uint_as_float(x[q]), c, -b));
-                            if (some_hidden) e = k + q < cols ? e : 0.0f;
-                            l += e;
-                            x[q] = __float_as_uint(e);
+                        for (int q = 0; q < 16; ++q) {
+                            float2 e = __ffma2_rn(make_float2(__uint_as_float(x[k + 2 * q]), __uint_as_float(x[k + 2 * q + 1])), make_float2(c, c), make_float2(b, b));
+                            e.x = ex2(e.x); e.y = ex2(e.y);
+                            sum[q & 1] = __fadd2_rn(sum[q & 1], e);
+                            y[q] = pack2<T>(e.x, e.y);
                         }
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) y[q] = pack2<T>(__uint_as_float(x[2 * q]), __uint_as_float(x[2 * q + 1]));
                         tmem_st16(s_at + k / 2, y);
                     }
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_wait_st();
                 }
                 if (key0 + MANY_KEYS > limit_all) {
@@ -379,12 +311,12 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         if (both) { mbar_arrive(&both_bar); ok = __all_sync(0xffffffffu, wait_or_abort(&both_bar, both_phase, abort_flag)); both_phase ^= 1; }
                         else { mbar_arrive(&alone_bar[s]); ok = __all_sync(0xffffffffu, wait_or_abort(&alone_bar[s], alone_phase, abort_flag)); alone_phase ^= 1; }
                     };
-                    const int there = seen - key0;           // a thread to a key
+                    const int there = u.seen - key0;         // a thread to a key
                     const bool looks = !both || s == 0;
                     uint32_t *found = special_sh[both ? 2 + both_phase : s];
                     if (looks) {
                         bool special = false;
-                        if (r < there && st.own) {
+                        if (r < there && u.own) {
 #pragma unroll
                             for (int ch = 0; ch < HD / 8; ++ch) special |= any_special<T>(lds_128(v_at + swizzled(r, ch)));
                         }
@@ -424,36 +356,171 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             ok = __all_sync(0xffffffffu, wait_or_abort(&o_bar[s], turn & 1, abort_flag));
             if (!ok) break;
             after_sync();
-            const bool whole = piece.n == piece.ut && st.own && !w.halves && group_of(p, piece.e - p.n_groups) < 0;      // nothing to join with
+            const bool whole = piece.n == piece.ut && !w.halves && alone(p, piece);          // nothing to join with
             const long long place = (line.tile[piece.e] + (long long)piece.h * piece.tiles + piece.t + blockIdx.x) * MANY_ROWS + s * HALF_ROWS + r;
+            // the other stream reads this one's queries, whose room the results pass through
+            if (w.halves && s == 0 && !__all_sync(0xffffffffu, wait_or_abort(&o_bar[1], turn & 1, abort_flag))) { ok = false; break; }
             if (warp_valid) {
-                const float inv = 1.0f / l;
-                uint4 *to = whole ? reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.d_out) + (long long)(row0 + i / p.G) * a.out_ld + (size_t)(piece.h * p.G + i % p.G) * HD)
-                                  : reinterpret_cast<uint4 *>(out.acc + place * HD);
+                // Through the room of the warp's own queries, 32 columns at a time: a thread holds a row, a store covers 128 bytes of four.
+                const float inv = whole ? 1.0f / l : 1.0f;
+                const long long out_off = (long long)row * a.out_ld + column;
+                const int rows = min(32, st.nr - (i - lane)), ch = lane & 7;
 #pragma unroll 1
                 for (int k = 0; k < HD; k += 32) {
+                    const uint32_t stage = q_tiles + s * Q_TILE + (k / 32) % NB * BLOCK64 + (warp & 3) * 4096;
                     uint32_t x[32];
                     tmem_ld32(o_at + k, x);
-                    if (!valid) continue;
-                    if (whole) {
-                        uint32_t y[16];
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) y[q] = pack2<T>(__uint_as_float(x[2 * q]) * inv, __uint_as_float(x[2 * q + 1]) * inv);
+                    for (int q = 0; q < 8; ++q)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((q ^ (lane & 7)) * 16)), "r"(x[4 * q]), "r"(x[4 * q + 1]),
+                                     "r"(x[4 * q + 2]), "r"(x[4 * q + 3]) : "memory");
+                    __syncwarp();
+                    float *acc = out.acc + (place - lane) * HD + k + ch * 4;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) to[k / 8 + q] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) to[k / 4 + q] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+                    for (int q = 0; q < 8; ++q) {
+                        const int k_row = 4 * q + (lane >> 3);
+                        const long long off = __shfl_sync(0xffffffffu, out_off, k_row);
+                        const float f = __shfl_sync(0xffffffffu, inv, k_row);
+                        const uint4 v = lds_128(stage + k_row * 128 + ((ch ^ (k_row & 7)) * 16));
+                        if (k_row < rows) {
+                            if (whole) {
+                                uint2 y;
+                                y.x = pack2<T>(__uint_as_float(v.x) * f, __uint_as_float(v.y) * f);
+                                y.y = pack2<T>(__uint_as_float(v.z) * f, __uint_as_float(v.w) * f);
+                                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.d_out) + off + k + ch * 4) = y;
+                            } else *reinterpret_cast<uint4 *>(acc + (long long)k_row * HD) = v;
+                        }
                     }
+                    __syncwarp();
                 }
                 if (valid && !whole) out.top[place] = make_float2(top, l);
             }
             before_sync();
-            if (w.halves && s == 0) ok = __all_sync(0xffffffffu, wait_or_abort(&o_bar[1], turn & 1, abort_flag));       // the other stream reads this one's queries
             ++turn;
             item += 2 * piece.n;
         }
         if (!ok && lane == 0) give_up();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // ---- pages into the ring ----
+            const int box = min(a.page, MANY_KEYS), page_shift = 31 - __clz(a.page), boxes = MANY_KEYS / box;
+            asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
+            uint32_t item = 0;
+            bool outside = false, ok = true;
+            Walk walk(p, line, blockIdx.x);
+            Piece piece;
+            while (ok && walk.next(p, line, cut, piece)) {
+                const Streams w = streams_of(p, cut, piece);
+                const int n = piece.n;
+                auto load = [&](int unit, bool values) {         // by the whole warp
+                    const int slot = item % m.slots;
+                    const uint32_t phase = (item / m.slots) & 1;
+                    ++item;
+                    const Part u = part_at(a, p, cut, piece, unit);
+                    const int there = min(boxes, (u.seen - u.key0 + box - 1) / box);
+                    const int mine = lane / NB, part = lane % NB, key = u.key0 + mine * box;
+                    int id = mine < there ? __ldg(u.table + (key >> page_shift)) : 0;
+                    if (id < 0 || id >= a.n_pages) { outside = true; id = -1; }
+                    if (!__all_sync(0xffffffffu, wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag))) { ok = false; return; }
+                    if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)there * box * 128 * NB);
+                    __syncwarp();
+                    if (mine < there)                            // an id of -1 is outside the map and reads as zeros
+                        tma_load_3d(ring + slot * SLOT + part * BLOCK64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
+                                    id < 0 ? -1 : id * a.n_kv + piece.h, &full_bar[slot]);
+                };
+                if (w.halves) {
+                    load(0, false);
+                    if (ok && n > 1) load(1, false);
+                    for (int j = 0; j < n && ok; ++j) {
+                        load(j, true);
+                        if (ok && j + 2 < n) load(j + 2, false);
+                    }
+                } else {
+                    for (int j = 0; j < n && ok; ++j) {
+                        load(j, false);
+                        if (ok) load(j, true);
+                    }
+                }
+            }
+            if (!ok) give_up();
+            if (outside && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
+        } else if (warp == 1) {
+            // ---- the products ----
+            if (lane == 0) {
+                uint32_t item = 0, turn = 0, p_phase[2] = {0, 0};
+                bool ok = true;
+                Walk walk(p, line, blockIdx.x);
+                Piece piece;
+                auto full = [&](uint32_t i) {
+                    if (ok && !wait_or_abort(&full_bar[i % m.slots], (i / m.slots) & 1, abort_flag)) ok = false;
+                    after_sync();
+                };
+                auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % m.slots]); };
+                while (ok && walk.next(p, line, cut, piece)) {
+                    const Streams w = streams_of(p, cut, piece);
+                    const int n = piece.n;
+                    for (int s = 0; s < 2 && ok; ++s) ok = wait_or_abort(&q_bar[s], turn & 1, abort_flag);
+                    ++turn;
+                    if (!ok) break;
+                    after_sync();
+                    auto scores = [&](int s, uint32_t i) {
+                        const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % m.slots) * SLOT;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const uint64_t qd = smem_desc_sw128(q + b * BLOCK64), kd = smem_desc_sw128(k + b * BLOCK64);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) umma_f16(tmem + S_COL + s * 128, qd + 2 * j, kd + 2 * j, IDESC_S, (b | j) != 0);
+                        }
+                        umma_commit(&s_bar[s]);
+                    };
+                    auto sums = [&](int s, uint32_t i) {
+                        if (!wait_or_abort(&p_bar[s], p_phase[s], abort_flag)) { ok = false; return; }
+                        p_phase[s] ^= 1;
+                        after_sync();
+                        const uint64_t vd = smem_desc_rows(ring + (i % m.slots) * SLOT, BLOCK64);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) umma_from_tmem(tmem + O_COL + s * 128, tmem + S_COL + s * 128 + 8 * j, vd + 128 * j, IDESC_O);
+                    };
+                    if (w.halves) {
+                        full(item);
+                        if (!ok) break;
+                        scores(0, item); release(item);
+                        if (n > 1) { full(item + 1); if (!ok) break; scores(1, item + 1); release(item + 1); }
+                        else umma_commit(&o_bar[1]);
+                        for (int j = 0; j < n && ok; ++j) {
+                            const uint32_t v = item + place_of_values(true, n, j);
+                            full(v);
+                            if (ok) sums(j & 1, v);
+                            if (!ok) break;
+                            release(v);
+                            if (j + 2 < n) { full(v + 1); if (!ok) break; scores(j & 1, v + 1); release(v + 1); }
+                            else umma_commit(&o_bar[j & 1]);
+                        }
+                    } else {
+                        full(item);
+                        if (!ok) break;
+                        if (w.units[0] > 0) scores(0, item); else umma_commit(&o_bar[0]);
+                        scores(1, item); release(item);
+                        for (int j = 0; j < n && ok; ++j) {
+                            const uint32_t v = item + 2 * j + 1;
+                            full(v);
+                            if (ok && j < w.units[0]) {
+                                sums(0, v);
+                                if (!ok) break;
+                                if (j + 1 < w.units[0]) { full(v + 1); if (!ok) break; scores(0, v + 1); } else umma_commit(&o_bar[0]);
+                            }
+                            if (ok) sums(1, v);
+                            if (!ok) break;
+                            release(v);
+                            if (j + 1 < n) { full(v + 1); if (!ok) break; scores(1, v + 1); release(v + 1); } else umma_commit(&o_bar[1]);
+                        }
+                    }
+                    item += 2 * n;
+                }
+                if (!ok) give_up();
+            }
+        }
     }
 
     before_sync();
@@ -479,7 +546,7 @@ bool pool_map(CUtensorMap *map, const void *pool, const b200_paged_attn_args &a,
 }
 
 template <typename T, int HD>
-int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st)
+int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st)
 {
     constexpr size_t SLOT = BLOCK64 * (HD / 64);
     const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), room = 227 * 1024 - 1024 - 1024;    // static memory, alignment
@@ -503,7 +570,7 @@ int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cud
     at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_many_kernel<T, HD>, mk, mv, a, cut, out, m);
+    e = cudaLaunchKernelEx(&cfg, attn_many_kernel<T, HD>, mk, mv, a, cut, out, m, big);
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
     return 0;
@@ -511,8 +578,8 @@ int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cud
 
 }  // namespace
 
-int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, cudaStream_t st)
+int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st)
 {
-    if (a.wtype == B200_WT_F16) return a.hd == 64 ? launch<__half, 64>(a, cut, out, st) : launch<__half, 128>(a, cut, out, st);
-    return a.hd == 64 ? launch<__nv_bfloat16, 64>(a, cut, out, st) : launch<__nv_bfloat16, 128>(a, cut, out, st);
+    if (a.wtype == B200_WT_F16) return a.hd == 64 ? launch<__half, 64>(a, cut, out, big, st) : launch<__half, 128>(a, cut, out, big, st);
+    return a.hd == 64 ? launch<__nv_bfloat16, 64>(a, cut, out, big, st) : launch<__nv_bfloat16, 128>(a, cut, out, big, st);
 }

@@ -254,6 +254,9 @@ def test_attention(pkg, dtype, n_q, n_kv, hd, page, total, new, groups, prefix):
     (8, 8, 128, 256, [2000, 17], [129, 17], [0, 2], [128]),
     (5, 1, 128, 16, [260, 4000], [260, 77], [0, 2], [1]),
     (128, 1, 64, 16, [1, 2, 500], [1, 2, 3], [0, 3], [777]),                     # more query heads to a key / value head than a tile has rows
+    (32, 8, 128, 16, [500, 700, 3, 90, 333], [1, 200, 1, 40, 31], [0, 4], [301]),         # portions and single tokens in one group
+    (16, 2, 64, 32, [40, 64, 9, 1000, 17], [1, 64, 2, 16, 17], [1, 5], [640]),
+    (8, 1, 128, 64, [16, 700, 16], [16, 500, 1], [0, 2, 3], [4000, 127]),
     (16, 8, 128, 16, [2] * 200 + [3000] * 24, [1] * 224, [0, 100, 224], [300, 90]),
 ])
 def test_attention_larger(pkg, dtype, n_q, n_kv, hd, page, total, new, groups, prefix):
