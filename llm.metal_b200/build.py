@@ -25,7 +25,7 @@ LIB_SYNTH = os.path.join(HERE, "libllmb200_synth.so")
 
 CU_SOURCES = ["pack.cu", "matvec.cu", "matvec_ext.cu", "matvec_ext_plain.cu", "matvec_streams.cu", "attention.cu", "decode_token.cu", "decode_token_narrow.cu", "lora_decode.cu", "batch_kernels.cu", "gemm_f32.cu", "gemm_tf32.cu", "gemm_pair.cu", "train_kernels.cu",
               "latent_attention.cu", "gqa_attention.cu", "gla.cu", "row_kernels.cu", "rows_matmul.cu", "prompt_rows.cu",
-              "paged_cache.cu", "paged_attention.cu", "paged_attention_many.cu"]
+              "paged_cache.cu", "paged_attention.cu"]
 C_SOURCES = ["weights.c", "decode_engine.c", "sft_engine.c", "batch_engine.c", "json.c", "tensor_file.c", "model_dir.c", "model_dir_common.c", "latent_model.c", "hybrid_model.c", "plain_rows.c"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

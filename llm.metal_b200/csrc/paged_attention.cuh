@@ -1,4 +1,4 @@
-// What the two forms of attention over pages share: elements of the cache's type, and the second form's launch.
+// What the kernels of attention over pages share: elements of the cache's type.
 #pragma once
 #include "paged_plan.cuh"
 
@@ -6,8 +6,6 @@
 
 #include <limits.h>
 #include <type_traits>
-
-extern unsigned long long g_b200_launches;
 
 namespace {
 
@@ -44,10 +42,4 @@ template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v
     return any;
 }
 
-// BIG_ROWS: a request of that many query rows fills a stream of attn_many_kernel by itself.
-constexpr int MANY_ROWS = 256, MANY_KEYS = 128, MANY_LEAST = 2, MANY_GAP = 3, BIG_ROWS = 128;
-
 }  // namespace
-
-// attn_many_kernel (paged_attention_many.cu): the sets of more than `lo` query rows, hd 64 or 128. One block to an SM.
-int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st);

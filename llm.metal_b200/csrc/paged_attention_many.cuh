@@ -1,4 +1,4 @@
-// Attention over pages for sets of many query rows (sm_100a): the prefix that a group shares, and the own tokens of requests that bring portions of prompts
+// Attention over pages for sets of many query rows: the prefix that a group shares, and the own tokens of requests that bring portions of prompts
 // (paged_plan.cuh). Both products run on tcgen05.
 //
 // A block works on two streams that take turns on the tensor core, so that one's softmax runs under the other's products: the two halves of a tile of 256 query
@@ -11,12 +11,13 @@
 //   warps 4-7   stream 0: queries into shared memory, softmax, results; warps 8-11 stream 1. A thread to a row.
 // Bound by memory for one tile of rows to a set (decode of a group), by the tensor core and the exponentials for several.
 // Every wait is bounded; on a timeout the block reports it, lets copies in flight land, frees its tensor memory and returns.
+#pragma once
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
 namespace {
 
-constexpr int MANY_THREADS = 384, HALF_ROWS = MANY_ROWS / 2, MOST_SLOTS = 8;
+constexpr int MANY_ROWS = Cut<1>::ROWS, MANY_KEYS = Cut<1>::KEYS, MANY_THREADS = 384, HALF_ROWS = MANY_ROWS / 2, MOST_SLOTS = 8;
 constexpr uint32_t BLOCK64 = MANY_KEYS * 128;                // 128 rows of 64 numbers
 constexpr int S_COL = 0, O_COL = 256;                        // tensor memory: S of stream s at 128 s, O at 256 + 128 s
 
@@ -135,54 +136,45 @@ template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at
     tmem_wait_st();
 }
 
-struct ManyArgs { int slots, plan_off; };
-
 // Which units of a piece a stream has.
 struct Streams {
     bool halves;                         // one tile of rows, every other unit to a stream
     int units[2];
 };
-__device__ __forceinline__ Streams streams_of(const Plan &p, const Cut &c, const Piece &q)
+__device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q)
 {
     Streams w;
     const int valid = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS);
     w.halves = valid <= HALF_ROWS;
     if (w.halves) { w.units[0] = (q.n + 1) / 2; w.units[1] = q.n / 2; return w; }
-    const int seen = q.s.own ? q.s.keys - q.s.rows + (q.t * MANY_ROWS + HALF_ROWS - 1) / p.G + 1 : q.s.keys;
-    w.units[0] = max(0, min(q.n, units_before_own(q.s, c) + (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
+    const int seen = q.s.own ? q.s.keys - q.s.rows + over(q.t * MANY_ROWS + HALF_ROWS - 1, p.shape.by_g) + 1 : q.s.keys;
+    w.units[0] = max(0, min(q.n, units_before_own<1>(q.s) + (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
     w.units[1] = q.n;
     return w;
 }
 // The order in which keys and values of a piece of n units pass through the ring: K0 V0 K1 V1 .. for two halves of rows; K0 K1 V0 K2 V1 K3 .. for every other unit.
 __device__ __forceinline__ int place_of_values(bool halves, int n, int j) { return halves ? 2 + j + min(j, n - 2) : 2 * j + 1; }
 
+// A block's stretch of the second line. `base`: two tiles of queries and `slots` places of keys or values, 1024-byte aligned.
 template <typename T, int HD>
-__global__ void __launch_bounds__(MANY_THREADS, 1)
-attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ b200_paged_attn_args a, const Cut cut,
-                 const Pieces out, const ManyArgs m, int big)
+__device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUtensorMap &map_v, const b200_paged_attn_args &a, const Plan &p, const Pieces &out, char *base, int slots)
 {
     constexpr int NB = HD / 64;
     constexpr uint32_t SLOT = BLOCK64 * NB, Q_TILE = BLOCK64 * NB;
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(MANY_KEYS >> 3) << 17) | (8u << 24);
     constexpr uint32_t IDESC_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
-    extern __shared__ __align__(1024) char smem[];
     __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2], p_bar[2], o_bar[2], alone_bar[2], both_bar;
-    __shared__ long long red[32];
-    __shared__ int red_t[32];
-    __shared__ Plan plan_sh;
-    __shared__ Line line_sh;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_sh;
     __shared__ uint32_t special_sh[4][4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &abort_sh;
-    char *base = smem + ((1024 - (smem_u32(smem) & 1023)) & 1023);
     const uint32_t q_tiles = smem_u32(base), ring = q_tiles + 2 * Q_TILE;
 
     if (threadIdx.x == 0) {
         abort_sh = 0;
-        for (int s = 0; s < m.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int s = 0; s < slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&q_bar[s], 128); mbar_init(&s_bar[s], 1); mbar_init(&p_bar[s], 128); mbar_init(&o_bar[s], 1); mbar_init(&alone_bar[s], 128);
         }
@@ -198,17 +190,6 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __syncthreads();
     after_sync();
     const uint32_t tmem = tmem_sh;
-    pdl_wait();
-    pdl_launch_dependents();                                 // after the wait: attn_few_kernel starts on this and waits for nothing else
-    {
-        Plan plan;
-        Line laid;
-        if (!load_plan(a, plan, base + m.plan_off, 1, big, red_t) || !lay_line(a, plan, cut, 0, out.workers, laid, red, red_t)) laid.units = laid.per = 0;
-        if (threadIdx.x == 0) { plan_sh = plan; line_sh = laid; }
-        __syncthreads();
-    }
-    const Plan &p = plan_sh;                                 // in shared memory: registers are for the scores
-    const Line &line = line_sh;
     auto give_up = [&]() { if (!*abort_flag) { *abort_flag = 1; if (a.d_status) atomicOr(a.d_status, B200_PAGED_TIMED_OUT); } };
 
     // Registers: 168 a thread at the launch, 384 threads; 72 for four warps and 216 for the eight with a row of scores a thread are as many.
@@ -221,15 +202,16 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         uint32_t turn = 0, item = 0, s_phase = 0, alone_phase = 0, both_phase = 0;
         bool ok = true;
-        Walk walk(p, line, blockIdx.x);
+        Walk<1> walk(p, blockIdx.x);
         Piece piece;
-        while (ok && walk.next(p, line, cut, piece)) {
-            const Streams w = streams_of(p, cut, piece);
+        while (ok && walk.next(p, piece)) {
+            const Streams w = streams_of(p, piece);
             const Set &st = piece.s;
             const int i0 = piece.t * MANY_ROWS, i = i0 + (w.halves ? 0 : s * HALF_ROWS) + r, mine = w.units[s];
             const bool valid = i < st.nr, warp_valid = __any_sync(0xffffffffu, valid);
-            const int row = row_at(p, piece.e, min(i, st.nr - 1) / p.G);
-            const size_t column = (size_t)(piece.h * p.G + min(i, st.nr - 1) % p.G) * HD;
+            const Div by_g = p.shape.by_g;
+            const int last = min(i, st.nr - 1), local = over(last, by_g), row = row_at(p, piece.e, local);
+            const int column = (piece.h * by_g.d + last - local * by_g.d) * HD;
             // a warp's rows, HD / 8 lanes to each so that whole lines are read; all loads before the first store
             constexpr int CH = HD / 8, RL = 32 / CH;         // 16-byte chunks of a row, rows of a load
             const long long q_off = (long long)row * a.q_ld + column;
@@ -257,10 +239,10 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             float top = -INFINITY, l = 0.0f;
             for (int j = 0; j < mine; ++j) {
                 const int unit = w.halves ? 2 * j + s : j;
-                const Part u = part_at(a, p, cut, piece, unit);
+                const Part u = part_at<1>(a, p, piece, unit);
                 // keys that this row sees, that the first row of this warp sees, that the first row of the whole tile sees (all rows see)
-                const int key0 = u.key0, limit = u.own ? st.keys - st.rows + min(i, st.nr - 1) / p.G + 1 : u.seen, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
-                const int limit_all = u.own ? st.keys - st.rows + i0 / p.G + 1 : u.seen;
+                const int key0 = u.key0, limit = u.own ? st.keys - st.rows + local + 1 : u.seen, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
+                const int limit_all = u.own ? st.keys - st.rows + over(i0, by_g) + 1 : u.seen;
                 if (!__all_sync(0xffffffffu, wait_or_abort(&s_bar[s], s_phase, abort_flag))) { ok = false; break; }
                 s_phase ^= 1;
                 after_sync();
@@ -304,8 +286,8 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 if (key0 + MANY_KEYS > limit_all) {
                     // Not all rows see all of these keys: zero weights must not meet infinities or NaN. Values behind the last seen key are made zero; of those
                     // that some rows see, the ones that are not finite are added row by row and then made zero too.
-                    const uint32_t v_item = item + place_of_values(w.halves, piece.n, unit), v_at = ring + (v_item % m.slots) * SLOT;
-                    if (!__all_sync(0xffffffffu, wait_or_abort(&full_bar[v_item % m.slots], (v_item / m.slots) & 1, abort_flag))) { ok = false; break; }
+                    const uint32_t v_item = item + place_of_values(w.halves, piece.n, unit), v_at = ring + (v_item % slots) * SLOT;
+                    if (!__all_sync(0xffffffffu, wait_or_abort(&full_bar[v_item % slots], (v_item / slots) & 1, abort_flag))) { ok = false; break; }
                     const bool both = !w.halves && unit < w.units[0];
                     auto meet = [&]() {                      // of all threads that read this unit
                         if (both) { mbar_arrive(&both_bar); ok = __all_sync(0xffffffffu, wait_or_abort(&both_bar, both_phase, abort_flag)); both_phase ^= 1; }
@@ -357,7 +339,7 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (!ok) break;
             after_sync();
             const bool whole = piece.n == piece.ut && !w.halves && alone(p, piece);          // nothing to join with
-            const long long place = (line.tile[piece.e] + (long long)piece.h * piece.tiles + piece.t + blockIdx.x) * MANY_ROWS + s * HALF_ROWS + r;
+            const long long place = (long long)(p.tile[1][piece.e] + piece.h * piece.tiles + piece.t + (int)blockIdx.x) * MANY_ROWS + s * HALF_ROWS + r;
             // the other stream reads this one's queries, whose room the results pass through
             if (w.halves && s == 0 && !__all_sync(0xffffffffu, wait_or_abort(&o_bar[1], turn & 1, abort_flag))) { ok = false; break; }
             if (warp_valid) {
@@ -408,16 +390,16 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
             uint32_t item = 0;
             bool outside = false, ok = true;
-            Walk walk(p, line, blockIdx.x);
+            Walk<1> walk(p, blockIdx.x);
             Piece piece;
-            while (ok && walk.next(p, line, cut, piece)) {
-                const Streams w = streams_of(p, cut, piece);
+            while (ok && walk.next(p, piece)) {
+                const Streams w = streams_of(p, piece);
                 const int n = piece.n;
                 auto load = [&](int unit, bool values) {         // by the whole warp
-                    const int slot = item % m.slots;
-                    const uint32_t phase = (item / m.slots) & 1;
+                    const int slot = item % slots;
+                    const uint32_t phase = (item / slots) & 1;
                     ++item;
-                    const Part u = part_at(a, p, cut, piece, unit);
+                    const Part u = part_at<1>(a, p, piece, unit);
                     const int there = min(boxes, (u.seen - u.key0 + box - 1) / box);
                     const int mine = lane / NB, part = lane % NB, key = u.key0 + mine * box;
                     int id = mine < there ? __ldg(u.table + (key >> page_shift)) : 0;
@@ -450,22 +432,22 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (lane == 0) {
                 uint32_t item = 0, turn = 0, p_phase[2] = {0, 0};
                 bool ok = true;
-                Walk walk(p, line, blockIdx.x);
+                Walk<1> walk(p, blockIdx.x);
                 Piece piece;
                 auto full = [&](uint32_t i) {
-                    if (ok && !wait_or_abort(&full_bar[i % m.slots], (i / m.slots) & 1, abort_flag)) ok = false;
+                    if (ok && !wait_or_abort(&full_bar[i % slots], (i / slots) & 1, abort_flag)) ok = false;
                     after_sync();
                 };
-                auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % m.slots]); };
-                while (ok && walk.next(p, line, cut, piece)) {
-                    const Streams w = streams_of(p, cut, piece);
+                auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % slots]); };
+                while (ok && walk.next(p, piece)) {
+                    const Streams w = streams_of(p, piece);
                     const int n = piece.n;
                     for (int s = 0; s < 2 && ok; ++s) ok = wait_or_abort(&q_bar[s], turn & 1, abort_flag);
                     ++turn;
                     if (!ok) break;
                     after_sync();
                     auto scores = [&](int s, uint32_t i) {
-                        const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % m.slots) * SLOT;
+                        const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % slots) * SLOT;
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             const uint64_t qd = smem_desc_sw128(q + b * BLOCK64), kd = smem_desc_sw128(k + b * BLOCK64);
@@ -478,7 +460,7 @@ attn_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         if (!wait_or_abort(&p_bar[s], p_phase[s], abort_flag)) { ok = false; return; }
                         p_phase[s] ^= 1;
                         after_sync();
-                        const uint64_t vd = smem_desc_rows(ring + (i % m.slots) * SLOT, BLOCK64);
+                        const uint64_t vd = smem_desc_rows(ring + (i % slots) * SLOT, BLOCK64);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) umma_from_tmem(tmem + O_COL + s * 128, tmem + S_COL + s * 128 + 8 * j, vd + 128 * j, IDESC_O);
                     };
@@ -545,41 +527,4 @@ bool pool_map(CUtensorMap *map, const void *pool, const b200_paged_attn_args &a,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD>
-int launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st)
-{
-    constexpr size_t SLOT = BLOCK64 * (HD / 64);
-    const size_t plan = plan_bytes(a.n_req, a.n_groups, 1), room = 227 * 1024 - 1024 - 1024;    // static memory, alignment
-    ManyArgs m;
-    m.slots = (int)((room - 2 * SLOT - plan) / SLOT);
-    if (m.slots > MOST_SLOTS) m.slots = MOST_SLOTS;
-    m.plan_off = (int)((2 + m.slots) * SLOT);
-    const size_t smem = m.plan_off + plan + 1024;
-    const int box = a.page < MANY_KEYS ? a.page : MANY_KEYS;
-    CUtensorMap mk, mv;
-    if (!pool_map(&mk, a.d_k_pool, a, box) || !pool_map(&mv, a.d_v_pool, a, box)) return B200_E_STATE;
-    cudaError_t e = cudaFuncSetAttribute(attn_many_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)out.workers);
-    cfg.blockDim = dim3(MANY_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = a.use_pdl != 0;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_many_kernel<T, HD>, mk, mv, a, cut, out, m, big);
-    if (e != cudaSuccess) return (int)e;
-    ++g_b200_launches;
-    return 0;
-}
-
 }  // namespace
-
-int attn_many_launch(const b200_paged_attn_args &a, const Cut &cut, const Pieces &out, int big, cudaStream_t st)
-{
-    if (a.wtype == B200_WT_F16) return a.hd == 64 ? launch<__half, 64>(a, cut, out, big, st) : launch<__half, 128>(a, cut, out, big, st);
-    return a.hd == 64 ? launch<__nv_bfloat16, 64>(a, cut, out, big, st) : launch<__nv_bfloat16, 128>(a, cut, out, big, st);
-}
