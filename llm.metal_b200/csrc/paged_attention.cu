@@ -154,7 +154,7 @@ Layout layout_of(const b200_paged_attn_args &a)
     Layout L = {};
     L.shape.by_g = div_of((int)G); L.shape.by_kv = div_of(a.n_kv);
     L.shape.few_most = wide ? FEW_MOST : INT_MAX; L.shape.big = wide ? BIG_ROWS : INT_MAX;
-    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 14 : 10;
+    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 7 : 5;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
     const long long few_tiles = sets * ((FEW_MOST + FEW_ROWS - 1) / FEW_ROWS), full = (all + FEW_ROWS - 1) / FEW_ROWS + sets;
     const long long few_slots = (wide && few_tiles < full ? few_tiles : full) * a.n_kv + L.shape.blocks * L.shape.few_warps;
@@ -180,10 +180,10 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     Room room = {0, (int)rings};
     CUtensorMap map_k = {}, map_v = {};
     if constexpr (HD <= 128) {
-        constexpr size_t SLOT = BLOCK64 * (HD / 64);
-        const size_t left = 227 * 1024 - 1024 - 2048 - plan - 2 * SLOT;      // but for the alignment, the static memory, the plan and the queries
+        constexpr size_t SLOT = KEY64 * (HD / 64), QUERIES = 2 * QUERY64 * (HD / 64);
+        const size_t left = 227 * 1024 - 1024 - 2048 - plan - QUERIES;      // but for the alignment, the static memory, the plan and the queries
         room.slots = (int)(left / SLOT) < MOST_SLOTS ? (int)(left / SLOT) : MOST_SLOTS;
-        if ((2 + room.slots) * SLOT > rings) room.plan_off = (int)((2 + room.slots) * SLOT);
+        if (QUERIES + room.slots * SLOT > rings) room.plan_off = (int)(QUERIES + room.slots * SLOT);
         const int box = a.page < MANY_KEYS ? a.page : MANY_KEYS;
         if (!pool_map(&map_k, a.d_k_pool, a, box) || !pool_map(&map_v, a.d_v_pool, a, box)) return B200_E_STATE;
     }

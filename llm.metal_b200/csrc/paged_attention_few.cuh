@@ -54,7 +54,8 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
         const int e = piece.e, h = piece.h, t = piece.t, k0 = piece.k0, n = piece.n;
         const int i0 = t * FEW_ROWS, valid = min(FEW_ROWS, s.nr - i0);
         const int seen = seen_by<0>(p, s, t), seen_first = s.own ? s.keys - s.rows + over(i0, by_g) + 1 : s.keys;
-        const int *table = part_at<0>(a, p, piece, 0).table;
+        const Keys keys = keys_of<0>(a, p, piece);                // (none comes before a request's own here)
+        const int *table = s.own ? keys.table : keys.prefix;
         int limit[2], row_of[2], column[2];
         uint32_t q[CH / 2][4];
 #pragma unroll

@@ -2,12 +2,13 @@
 // (paged_plan.cuh). Both products run on tcgen05.
 //
 // A block works on two streams that take turns on the tensor core, so that one's softmax runs under the other's products: the two halves of a tile of 256 query
-// rows on the same keys, or, where a tile has 128 rows at most, the same rows on every other unit of 128 keys, each stream with a maximum, sum and result of its own.
-// Per unit and stream: S = Q K^T (128 x 128, tensor memory), the weights P = 2^(c S - m) back into S's place as 16-bit pairs, O += P V with P as the operand from
-// tensor memory and V as it lies, [key][hd] (the product's second operand along its rows). m is the largest score so far only as far as it must be: O is rescaled when it
-// is exceeded by a factor of 2^8, which both 16-bit types have room for.
+// rows on the same keys, or, where a tile has 128 rows at most, the same rows on every other unit of 64 keys, each stream with a maximum, sum and result of its own.
+// Per unit and stream: S = Q K^T (128 x 64, one of two places in tensor memory, so that the next scores are there when these are done with), the weights
+// P = 2^(c S - m) back into S's place as 16-bit pairs, O += P V with P as the operand from tensor memory and V as it lies, [key][hd] (the product's
+// second operand along its rows). m is the largest score so far only as far as it must be: O is rescaled when it is exceeded by a factor of 2^8, which both 16-bit
+// types have room for.
 //   warp 0      pages into a ring of shared memory: TMA, a box of 64 numbers by up to 128 tokens a lane, keys and values by turns
-//   warp 1      one lane issues the products
+//   warps 1, 2  the products of stream 0, of stream 1: one lane issues them
 //   warps 4-7   stream 0: queries into shared memory, softmax, results; warps 8-11 stream 1. A thread to a row.
 // Bound by memory for one tile of rows to a set (decode of a group), by the tensor core and the exponentials for several.
 // Every wait is bounded; on a timeout the block reports it, lets copies in flight land, frees its tensor memory and returns.
@@ -17,9 +18,9 @@
 
 namespace {
 
-constexpr int MANY_ROWS = Cut<1>::ROWS, MANY_KEYS = Cut<1>::KEYS, MANY_THREADS = 384, HALF_ROWS = MANY_ROWS / 2, MOST_SLOTS = 8;
-constexpr uint32_t BLOCK64 = MANY_KEYS * 128;                // 128 rows of 64 numbers
-constexpr int S_COL = 0, O_COL = 256;                        // tensor memory: S of stream s at 128 s, O at 256 + 128 s
+constexpr int MANY_ROWS = Cut<1>::ROWS, MANY_KEYS = Cut<1>::KEYS, MANY_THREADS = 384, HALF_ROWS = MANY_ROWS / 2, MOST_SLOTS = 12;
+constexpr uint32_t QUERY64 = HALF_ROWS * 128, KEY64 = MANY_KEYS * 128;       // 64 numbers of a tile's rows, of a unit's keys
+constexpr int S_COL = 0, O_COL = 256;                        // tensor memory: S of stream s at 128 s and 128 s + 64, O at 256 + 128 s
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar)
 {
@@ -51,35 +52,23 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) { tmem_st16(taddr, r); tmem_st16(taddr + 16, r + 16); }
-// 128 columns of the lanes' rows
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128])
+// 64 columns of the lanes' rows
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64])
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
-        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
-        "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
-        "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
-        "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-        : "r"(taddr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+                 "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr)
@@ -89,11 +78,20 @@ __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr)
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     return r;
 }
+// One lane of a converged warp. (By the whole warp up to here, so that addresses and descriptors stay in uniform registers, which is where the products take them from.)
+__device__ __forceinline__ bool one_lane()
+{
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t swizzled(int row, int ch) { return (ch >> 3) * BLOCK64 + row * 128 + (((ch & 7) ^ (row & 7)) * 16); }     // chunk ch of a row
+// chunk ch of a row of a tile whose 64 numbers a row lie `block` bytes apart
+__device__ __forceinline__ uint32_t swizzled(int row, int ch, uint32_t block) { return (ch >> 3) * block + row * 128 + (((ch & 7) ^ (row & 7)) * 16); }
 __device__ __forceinline__ void zero16(uint32_t at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory"); }
 
 // The rows' results times f: by the whole warp. Eight columns at a time: a row of scores is held meanwhile.
@@ -122,7 +120,7 @@ template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at
         tmem_ld32(o_at + k, x);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
-            const uint4 v = lds_128(v_at + swizzled(key, k / 8 + ch));
+            const uint4 v = lds_128(v_at + swizzled(key, k / 8 + ch, KEY64));
             const uint32_t word[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -136,50 +134,58 @@ template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at
     tmem_wait_st();
 }
 
-// Which units of a piece a stream has.
+// Which units of a piece a stream has, and the order in which the piece's keys and values pass through the ring: `lead` units of keys, then values and keys by turns.
 struct Streams {
     bool halves;                         // one tile of rows, every other unit to a stream
-    int units[2];
+    int units[2], n, lead;
+    __device__ __forceinline__ uint32_t values(int j) const { return lead + j + min(j, n - lead); }
 };
 __device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q)
 {
     Streams w;
-    const int valid = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS);
-    w.halves = valid <= HALF_ROWS;
+    w.n = q.n;
+    w.halves = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS) <= HALF_ROWS;
+    w.lead = min(q.n, w.halves ? 4 : 2);
     if (w.halves) { w.units[0] = (q.n + 1) / 2; w.units[1] = q.n / 2; return w; }
     const int seen = q.s.own ? q.s.keys - q.s.rows + over(q.t * MANY_ROWS + HALF_ROWS - 1, p.shape.by_g) + 1 : q.s.keys;
     w.units[0] = max(0, min(q.n, units_before_own<1>(q.s) + (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
     w.units[1] = q.n;
     return w;
 }
-// The order in which keys and values of a piece of n units pass through the ring: K0 V0 K1 V1 .. for two halves of rows; K0 K1 V0 K2 V1 K3 .. for every other unit.
-__device__ __forceinline__ int place_of_values(bool halves, int n, int j) { return halves ? 2 + j + min(j, n - 2) : 2 * j + 1; }
+
+// A place in the ring, and the phase of its barriers.
+struct Place {
+    int slot;
+    uint32_t phase;
+    __device__ __forceinline__ void next(int slots) { if (++slot == slots) { slot = 0; phase ^= 1; } }
+};
 
 // A block's stretch of the second line. `base`: two tiles of queries and `slots` places of keys or values, 1024-byte aligned.
 template <typename T, int HD>
 __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUtensorMap &map_v, const b200_paged_attn_args &a, const Plan &p, const Pieces &out, char *base, int slots)
 {
     constexpr int NB = HD / 64;
-    constexpr uint32_t SLOT = BLOCK64 * NB, Q_TILE = BLOCK64 * NB;
+    constexpr uint32_t SLOT = KEY64 * NB, Q_TILE = QUERY64 * NB;
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(MANY_KEYS >> 3) << 17) | (8u << 24);
     constexpr uint32_t IDESC_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
-    __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2], p_bar[2], o_bar[2], alone_bar[2], both_bar;
+    __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2][2], p_bar[2][2], o_bar[2][2], alone_bar[2], both_bar, both_done;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_sh;
-    __shared__ uint32_t special_sh[4][4];
+    __shared__ uint32_t special_sh[4][2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &abort_sh;
     const uint32_t q_tiles = smem_u32(base), ring = q_tiles + 2 * Q_TILE;
 
     if (threadIdx.x == 0) {
         abort_sh = 0;
-        for (int s = 0; s < slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int s = 0; s < slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 2); }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&q_bar[s], 128); mbar_init(&s_bar[s], 1); mbar_init(&p_bar[s], 128); mbar_init(&o_bar[s], 1); mbar_init(&alone_bar[s], 128);
+            mbar_init(&q_bar[s], 128); mbar_init(&s_bar[s][0], 1); mbar_init(&s_bar[s][1], 1); mbar_init(&alone_bar[s], 128);
+            for (int k = 0; k < 2; ++k) { mbar_init(&p_bar[s][k], 128); mbar_init(&o_bar[s][k], 1); }
         }
-        mbar_init(&both_bar, 256);
-        for (int i = 0; i < 16; ++i) special_sh[i >> 2][i & 3] = 0;
+        mbar_init(&both_bar, 256); mbar_init(&both_done, 2);
+        for (int i = 0; i < 8; ++i) special_sh[i >> 1][i & 1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -197,10 +203,10 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- a stream's rows ----
         const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;       // stream, row of its tile = lane of tensor memory
-        const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), s_at = tm + S_COL + s * 128, o_at = tm + O_COL + s * 128;
+        const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), o_at = tm + O_COL + s * 128;
         const float c = fabsf(a.scale) * 1.4426950408889634f;            // the sign goes into the queries
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        uint32_t turn = 0, item = 0, s_phase = 0, alone_phase = 0, both_phase = 0;
+        uint32_t turn = 0, item = 0, s_phase = 0, even = 0, odd = 0, alone_phase = 0, both_phase = 0;      // even, odd: products with weights of the first and of the second place, before this piece
         bool ok = true;
         Walk<1> walk(p, blockIdx.x);
         Piece piece;
@@ -212,6 +218,9 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             const Div by_g = p.shape.by_g;
             const int last = min(i, st.nr - 1), local = over(last, by_g), row = row_at(p, piece.e, local);
             const int column = (piece.h * by_g.d + last - local * by_g.d) * HD;
+            // own keys that this row sees, that the first row of this warp sees, that the first row of the whole tile sees (all rows see)
+            const Keys keys = keys_of<1>(a, p, piece);
+            const int own_limit = st.keys - st.rows + local + 1, own_warp = __shfl_sync(0xffffffffu, own_limit, 0), own_all = st.keys - st.rows + over(i0, by_g) + 1;
             // a warp's rows, HD / 8 lanes to each so that whole lines are read; all loads before the first store
             constexpr int CH = HD / 8, RL = 32 / CH;         // 16-byte chunks of a row, rows of a load
             const long long q_off = (long long)row * a.q_ld + column;
@@ -224,7 +233,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                 }
 #pragma unroll
                 for (int k = 0; k < 32 / RL; ++k)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_tiles + s * Q_TILE + swizzled((warp & 3) * 32 + k * RL + lane / CH, lane % CH)),
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_tiles + s * Q_TILE + swizzled((warp & 3) * 32 + k * RL + lane / CH, lane % CH, QUERY64)),
                                  "r"(v[k].x ^ flip), "r"(v[k].y ^ flip), "r"(v[k].z ^ flip), "r"(v[k].w ^ flip) : "memory");
             }
             async_proxy_fence();
@@ -237,32 +246,40 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             before_sync();
             mbar_arrive(&q_bar[s]);
             float top = -INFINITY, l = 0.0f;
+            auto settled = [&](int j) {                      // the sums of this piece's first j units are in O
+                if (j == 0) return true;
+                const int i = j - 1;
+                const bool there = __all_sync(0xffffffffu, wait_or_abort(&o_bar[s][i & 1], ((i & 1 ? odd : even) + i / 2) & 1, abort_flag));
+                after_sync();
+                return there;
+            };
             for (int j = 0; j < mine; ++j) {
-                const int unit = w.halves ? 2 * j + s : j;
-                const Part u = part_at<1>(a, p, piece, unit);
-                // keys that this row sees, that the first row of this warp sees, that the first row of the whole tile sees (all rows see)
-                const int key0 = u.key0, limit = u.own ? st.keys - st.rows + local + 1 : u.seen, limit_warp = __shfl_sync(0xffffffffu, limit, 0);
-                const int limit_all = u.own ? st.keys - st.rows + over(i0, by_g) + 1 : u.seen;
-                if (!__all_sync(0xffffffffu, wait_or_abort(&s_bar[s], s_phase, abort_flag))) { ok = false; break; }
-                s_phase ^= 1;
+                const int unit = w.halves ? 2 * j + s : j, place = j & 1;
+                const uint32_t s_at = tm + S_COL + s * 128 + place * 64;
+                const Part u = part_at<1>(keys, piece, unit);
+                const int key0 = u.key0, limit = u.own ? own_limit : u.seen, limit_warp = u.own ? own_warp : u.seen, limit_all = u.own ? own_all : u.seen;
+                if (!__all_sync(0xffffffffu, wait_or_abort(&s_bar[s][place], (s_phase >> place) & 1, abort_flag))) { ok = false; break; }
+                s_phase ^= 1u << place;
                 after_sync();
                 const bool some_hidden = key0 + MANY_KEYS > limit_warp;
                 const int cols = limit - key0;               // columns below this are seen
                 if (warp_valid) {
-                    uint32_t x[128];
-                    tmem_ld128(s_at, x);
+                    uint32_t x[64];
+                    tmem_ld64(s_at, x);
                     if (some_hidden) {
 #pragma unroll
-                        for (int q = 0; q < 128; ++q) x[q] = q < cols ? x[q] : 0xff800000u;
+                        for (int q = 0; q < 64; ++q) x[q] = q < cols ? x[q] : 0xff800000u;
                     }
                     float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int q = 0; q < 128; ++q) big4[q & 3] = fmaxf(big4[q & 3], __uint_as_float(x[q]));
+                    for (int q = 0; q < 64; ++q) big4[q & 3] = fmaxf(big4[q & 3], __uint_as_float(x[q]));
                     const float big = valid ? fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3])) * c : -INFINITY;   // (what lies in other rows must not decide)
                     if (__any_sync(0xffffffffu, big > top + 8.0f)) {     // (true too for the first)
                         const float higher = fmaxf(top, big), f = top == -INFINITY ? 0.0f : ex2(top - higher);
-                        // the products up to here are done: the score product that was waited for came after them
-                        if (__any_sync(0xffffffffu, top != -INFINITY)) scale_rows<HD>(o_at, f);
+                        if (__any_sync(0xffffffffu, top != -INFINITY)) {
+                            if (!settled(j)) { ok = false; break; }
+                            scale_rows<HD>(o_at, f);
+                        }
                         l *= f;
                         top = higher;
                     }
@@ -286,7 +303,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                 if (key0 + MANY_KEYS > limit_all) {
                     // Not all rows see all of these keys: zero weights must not meet infinities or NaN. Values behind the last seen key are made zero; of those
                     // that some rows see, the ones that are not finite are added row by row and then made zero too.
-                    const uint32_t v_item = item + place_of_values(w.halves, piece.n, unit), v_at = ring + (v_item % slots) * SLOT;
+                    const uint32_t v_item = item + w.values(unit), v_at = ring + (v_item % slots) * SLOT;
                     if (!__all_sync(0xffffffffu, wait_or_abort(&full_bar[v_item % slots], (v_item / slots) & 1, abort_flag))) { ok = false; break; }
                     const bool both = !w.halves && unit < w.units[0];
                     auto meet = [&]() {                      // of all threads that read this unit
@@ -298,31 +315,32 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     uint32_t *found = special_sh[both ? 2 + both_phase : s];
                     if (looks) {
                         bool special = false;
-                        if (r < there && u.own) {
+                        if (r < there && r < MANY_KEYS && u.own) {
 #pragma unroll
-                            for (int ch = 0; ch < HD / 8; ++ch) special |= any_special<T>(lds_128(v_at + swizzled(r, ch)));
+                            for (int ch = 0; ch < HD / 8; ++ch) special |= any_special<T>(lds_128(v_at + swizzled(r, ch, KEY64)));
                         }
                         const uint32_t word = __ballot_sync(0xffffffffu, special);
-                        if (lane == 0) found[warp & 3] = word;
-                        if (r >= there) {
+                        if (lane == 0 && r < MANY_KEYS) found[warp & 3] = word;
+                        if (r >= there && r < MANY_KEYS) {
 #pragma unroll
-                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch));
+                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch, KEY64));
                         }
                         async_proxy_fence();
                     }
                     meet();
                     if (!ok) break;
                     volatile uint32_t *marks = found;
-                    if (marks[0] | marks[1] | marks[2] | marks[3]) {     // the same for all who meet
+                    if (marks[0] | marks[1]) {                   // the same for all who meet
+                        if (!settled(j)) { ok = false; break; }
 #pragma unroll 1
                         for (int key = 0; key < MANY_KEYS; ++key)
                             if (marks[key >> 5] >> (key & 31) & 1) add_key<T, HD>(s_at, o_at, v_at, key, key < cols);
-                        const bool clear = looks && (marks[r >> 5] >> (r & 31) & 1);
+                        const bool clear = looks && r < MANY_KEYS && (marks[r >> 5] >> (r & 31) & 1);
                         meet();                              // nobody needs them any more
                         if (!ok) break;
                         if (clear) {
 #pragma unroll
-                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch));
+                            for (int ch = 0; ch < HD / 8; ++ch) zero16(v_at + swizzled(r, ch, KEY64));
                         }
                         async_proxy_fence();
                         meet();
@@ -330,18 +348,20 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     }
                 }
                 before_sync();
-                mbar_arrive(&p_bar[s]);
+                mbar_arrive(&p_bar[s][place]);
             }
             if (!ok) break;
 
             // ---- the piece's results ----
-            ok = __all_sync(0xffffffffu, wait_or_abort(&o_bar[s], turn & 1, abort_flag));
+            ok = settled(mine);
             if (!ok) break;
-            after_sync();
             const bool whole = piece.n == piece.ut && !w.halves && alone(p, piece);          // nothing to join with
             const long long place = (long long)(p.tile[1][piece.e] + piece.h * piece.tiles + piece.t + (int)blockIdx.x) * MANY_ROWS + s * HALF_ROWS + r;
-            // the other stream reads this one's queries, whose room the results pass through
-            if (w.halves && s == 0 && !__all_sync(0xffffffffu, wait_or_abort(&o_bar[1], turn & 1, abort_flag))) { ok = false; break; }
+            // All products of the piece are done: waited for once in every piece, so that no stream, not even one without units, runs two ahead of the products. Where
+            // the other stream reads this one's queries, before the results pass through their room.
+            auto finished = [&]() { return __all_sync(0xffffffffu, wait_or_abort(&both_done, turn & 1, abort_flag)); };
+            const bool early = w.halves && s == 0;
+            if (early && !finished()) { ok = false; break; }
             if (warp_valid) {
                 // Through the room of the warp's own queries, 32 columns at a time: a thread holds a row, a store covers 128 bytes of four.
                 const float inv = whole ? 1.0f / l : 1.0f;
@@ -349,7 +369,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                 const int rows = min(32, st.nr - (i - lane)), ch = lane & 7;
 #pragma unroll 1
                 for (int k = 0; k < HD; k += 32) {
-                    const uint32_t stage = q_tiles + s * Q_TILE + (k / 32) % NB * BLOCK64 + (warp & 3) * 4096;
+                    const uint32_t stage = q_tiles + s * Q_TILE + (k / 32) % NB * QUERY64 + (warp & 3) * 4096;
                     uint32_t x[32];
                     tmem_ld32(o_at + k, x);
 #pragma unroll
@@ -378,7 +398,9 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                 if (valid && !whole) out.top[place] = make_float2(top, l);
             }
             before_sync();
+            if (!early && !finished()) { ok = false; break; }
             ++turn;
+            even += (mine + 1) / 2; odd += mine / 2;
             item += 2 * piece.n;
         }
         if (!ok && lane == 0) give_up();
@@ -388,18 +410,19 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             // ---- pages into the ring ----
             const int box = min(a.page, MANY_KEYS), page_shift = 31 - __clz(a.page), boxes = MANY_KEYS / box;
             asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
-            uint32_t item = 0;
+            Place at = {0, 0};
             bool outside = false, ok = true;
             Walk<1> walk(p, blockIdx.x);
             Piece piece;
             while (ok && walk.next(p, piece)) {
                 const Streams w = streams_of(p, piece);
                 const int n = piece.n;
+                const Keys keys = keys_of<1>(a, p, piece);
                 auto load = [&](int unit, bool values) {         // by the whole warp
-                    const int slot = item % slots;
-                    const uint32_t phase = (item / slots) & 1;
-                    ++item;
-                    const Part u = part_at<1>(a, p, piece, unit);
+                    const int slot = at.slot;
+                    const uint32_t phase = at.phase;
+                    at.next(slots);
+                    const Part u = part_at<1>(keys, piece, unit);
                     const int there = min(boxes, (u.seen - u.key0 + box - 1) / box);
                     const int mine = lane / NB, part = lane % NB, key = u.key0 + mine * box;
                     int id = mine < there ? __ldg(u.table + (key >> page_shift)) : 0;
@@ -408,100 +431,106 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)there * box * 128 * NB);
                     __syncwarp();
                     if (mine < there)                            // an id of -1 is outside the map and reads as zeros
-                        tma_load_3d(ring + slot * SLOT + part * BLOCK64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
+                        tma_load_3d(ring + slot * SLOT + part * KEY64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
                                     id < 0 ? -1 : id * a.n_kv + piece.h, &full_bar[slot]);
                 };
-                if (w.halves) {
-                    load(0, false);
-                    if (ok && n > 1) load(1, false);
+                    for (int j = 0; j < w.lead && ok; ++j) load(j, false);
                     for (int j = 0; j < n && ok; ++j) {
                         load(j, true);
-                        if (ok && j + 2 < n) load(j + 2, false);
+                        if (ok && j + w.lead < n) load(j + w.lead, false);
                     }
-                } else {
-                    for (int j = 0; j < n && ok; ++j) {
-                        load(j, false);
-                        if (ok) load(j, true);
-                    }
-                }
             }
             if (!ok) give_up();
             if (outside && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
-        } else if (warp == 1) {
-            // ---- the products ----
-            if (lane == 0) {
-                uint32_t item = 0, turn = 0, p_phase[2] = {0, 0};
-                bool ok = true;
-                Walk<1> walk(p, blockIdx.x);
-                Piece piece;
-                auto full = [&](uint32_t i) {
-                    if (ok && !wait_or_abort(&full_bar[i % slots], (i / slots) & 1, abort_flag)) ok = false;
+        } else if (warp < 3) {
+            // ---- the products of a stream ----
+            // A division or an address made anew for each step would keep the tensor core waiting. Places in the ring are counted, descriptors are the
+            // first place's plus an offset, the whole warp follows and one lane issues.
+            const int s = warp - 1;
+            uint32_t turn = 0, p_phase = 0;
+            bool ok = true;
+            Walk<1> walk(p, blockIdx.x);
+            Piece piece;
+            Place at = {0, 0};
+            const uint64_t k_desc = smem_desc_sw128(ring), v_desc = smem_desc_rows(ring, KEY64);
+            const uint32_t s_at = tmem + S_COL + s * 128, o_at = tmem + O_COL + s * 128;
+            auto arrived = [&](uint64_t *bar, uint32_t phase) { return (bool)__all_sync(0xffffffffu, wait_or_abort(bar, phase, abort_flag)); };
+            while (ok && walk.next(p, piece)) {
+                const Streams w = streams_of(p, piece);
+                const int n = uniform(piece.n), mine = uniform(w.units[s]), lead = uniform(w.lead), halves = uniform(w.halves);
+                const uint64_t q_desc = smem_desc_sw128(q_tiles + (halves ? 0 : s * Q_TILE));
+                ok = arrived(&q_bar[0], turn & 1) && arrived(&q_bar[1], turn & 1);
+                ++turn;
+                if (!ok) break;
+                after_sync();
+                // A place is free again when both streams have said so, a stream that has no use for it too; the only reader of one says it twice.
+                auto scores = [&](int place, const Place &k) {
+                    if (!ok || !(ok = arrived(&full_bar[k.slot], k.phase))) return;
                     after_sync();
+                    const uint64_t kd = k_desc + k.slot * (SLOT >> 4);
+                    if (one_lane()) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) umma_f16(s_at + place * 64, q_desc + b * (QUERY64 >> 4) + 2 * x, kd + b * (KEY64 >> 4) + 2 * x, IDESC_S, (b | x) != 0);
+                        umma_commit(&s_bar[s][place]);
+                        umma_commit(&empty_bar[k.slot]);
+                        if (halves) umma_commit(&empty_bar[k.slot]);
+                    }
+                    __syncwarp();
                 };
-                auto release = [&](uint32_t i) { umma_commit(&empty_bar[i % slots]); };
-                while (ok && walk.next(p, piece)) {
-                    const Streams w = streams_of(p, piece);
-                    const int n = piece.n;
-                    for (int s = 0; s < 2 && ok; ++s) ok = wait_or_abort(&q_bar[s], turn & 1, abort_flag);
-                    ++turn;
-                    if (!ok) break;
+                auto sums = [&](int place, const Place &v) {
+                    if (!ok || !(ok = arrived(&full_bar[v.slot], v.phase) && arrived(&p_bar[s][place], (p_phase >> place) & 1))) return;
+                    p_phase ^= 1u << place;
                     after_sync();
-                    auto scores = [&](int s, uint32_t i) {
-                        const uint32_t q = q_tiles + (w.halves ? 0 : s * Q_TILE), k = ring + (i % slots) * SLOT;
+                    const uint64_t vd = v_desc + v.slot * (SLOT >> 4);
+                    if (one_lane()) {
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const uint64_t qd = smem_desc_sw128(q + b * BLOCK64), kd = smem_desc_sw128(k + b * BLOCK64);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) umma_f16(tmem + S_COL + s * 128, qd + 2 * j, kd + 2 * j, IDESC_S, (b | j) != 0);
-                        }
-                        umma_commit(&s_bar[s]);
-                    };
-                    auto sums = [&](int s, uint32_t i) {
-                        if (!wait_or_abort(&p_bar[s], p_phase[s], abort_flag)) { ok = false; return; }
-                        p_phase[s] ^= 1;
-                        after_sync();
-                        const uint64_t vd = smem_desc_rows(ring + (i % slots) * SLOT, BLOCK64);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) umma_from_tmem(tmem + O_COL + s * 128, tmem + S_COL + s * 128 + 8 * j, vd + 128 * j, IDESC_O);
-                    };
-                    if (w.halves) {
-                        full(item);
-                        if (!ok) break;
-                        scores(0, item); release(item);
-                        if (n > 1) { full(item + 1); if (!ok) break; scores(1, item + 1); release(item + 1); }
-                        else umma_commit(&o_bar[1]);
-                        for (int j = 0; j < n && ok; ++j) {
-                            const uint32_t v = item + place_of_values(true, n, j);
-                            full(v);
-                            if (ok) sums(j & 1, v);
-                            if (!ok) break;
-                            release(v);
-                            if (j + 2 < n) { full(v + 1); if (!ok) break; scores(j & 1, v + 1); release(v + 1); }
-                            else umma_commit(&o_bar[j & 1]);
-                        }
-                    } else {
-                        full(item);
-                        if (!ok) break;
-                        if (w.units[0] > 0) scores(0, item); else umma_commit(&o_bar[0]);
-                        scores(1, item); release(item);
-                        for (int j = 0; j < n && ok; ++j) {
-                            const uint32_t v = item + 2 * j + 1;
-                            full(v);
-                            if (ok && j < w.units[0]) {
-                                sums(0, v);
-                                if (!ok) break;
-                                if (j + 1 < w.units[0]) { full(v + 1); if (!ok) break; scores(0, v + 1); } else umma_commit(&o_bar[0]);
-                            }
-                            if (ok) sums(1, v);
-                            if (!ok) break;
-                            release(v);
-                            if (j + 1 < n) { full(v + 1); if (!ok) break; scores(1, v + 1); release(v + 1); } else umma_commit(&o_bar[1]);
+                        for (int x = 0; x < 4; ++x) umma_from_tmem(o_at, s_at + place * 64 + 8 * x, vd + 128 * x, IDESC_O);
+                        umma_commit(&o_bar[s][place]);
+                        umma_commit(&empty_bar[v.slot]);
+                        if (halves) umma_commit(&empty_bar[v.slot]);
+                    }
+                    __syncwarp();
+                };
+                auto pass = [&](const Place &x) {            // (arrived first: the word is for this occupant)
+                    if (!ok || !(ok = arrived(&full_bar[x.slot], x.phase))) return;
+                    if (lane == 0) mbar_arrive(&empty_bar[x.slot]);
+                    __syncwarp();
+                };
+                if (halves) {
+#pragma unroll 1
+                    for (int u = 0; u < lead; ++u, at.next(slots))
+                        if ((u & 1) == s) scores(u >> 1, at);
+#pragma unroll 1
+                    for (int u = 0; u < n && ok; ++u) {
+                        if ((u & 1) == s) sums((u >> 1) & 1, at);
+                        at.next(slots);
+                        if (u + 4 < n) {
+                            if ((u & 1) == s) scores((u >> 1) & 1, at);
+                            at.next(slots);
                         }
                     }
-                    item += 2 * n;
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < lead; ++j, at.next(slots)) {
+                        if (j < mine) scores(j, at); else pass(at);
+                    }
+#pragma unroll 1
+                    for (int j = 0; j < n && ok; ++j) {
+                        if (j < mine) sums(j & 1, at); else pass(at);
+                        at.next(slots);
+                        if (j + 2 < n) {
+                            if (j + 2 < mine) scores(j & 1, at); else pass(at);
+                            at.next(slots);
+                        }
+                    }
                 }
-                if (!ok) give_up();
+                if (!ok) break;
+                if (one_lane()) umma_commit(&both_done);
+                __syncwarp();
             }
+            if (!ok && lane == 0) give_up();
         }
     }
 

@@ -2,7 +2,7 @@
 // up to their own place, and a group's prefix, which all rows of the group see whole. (A request whose rows fill tiles by themselves meets the prefix and its own
 // tokens in one set: there is nothing to share then, and nothing to join.) A set's query rows are (row, query head of the key / value head) pairs, in that
 // order. Sets of few query rows go to single warps, in tiles of 16 rows and units of 16 keys; sets of many go to the tensor cores' wide form, in tiles
-// of 256 rows and units of 128 keys (the two ways).
+// of 256 rows and units of 64 keys (the two ways).
 //
 // All units of a way's sets lie on one line: set after set, and in it key / value head after head, tile after tile, with a gap before each tile for what
 // starting and storing it costs. The SMs are divided between the ways by the work on their lines, and a way's workers take equal stretches of its line,
@@ -44,7 +44,7 @@ namespace {
 // The two ways: rows of a tile, keys of a unit, fewest units of a worker, units' worth of a gap.
 template <int WAY> struct Cut;
 template <> struct Cut<0> { static constexpr int ROWS = 16, KEYS = 16, LEAST = 4, GAP = 1; };
-template <> struct Cut<1> { static constexpr int ROWS = 256, KEYS = 128, LEAST = 2, GAP = 3; };
+template <> struct Cut<1> { static constexpr int ROWS = 256, KEYS = 64, LEAST = 4, GAP = 6; };
 
 // What a block knows of the step, in shared memory.
 struct Plan {
@@ -324,15 +324,24 @@ template <int WAY> struct Walk {
     }
 };
 
+// Where the keys of a piece lie: in the prefix's pages, or behind `first` units of them in the request's own, and how many of each the tile's last row sees.
+struct Keys {
+    const int *prefix, *table;
+    int first, before, seen;
+};
+template <int WAY> __device__ __forceinline__ Keys keys_of(const b200_paged_attn_args &a, const Plan &p, const Piece &q)
+{
+    if (!q.s.own) return {a.d_prefix_table + (size_t)q.e * a.prefix_ld, nullptr, INT_MAX, q.s.keys, 0};
+    const int r = q.e - a.n_groups;
+    return {q.s.before ? a.d_prefix_table + (size_t)group_of(p, r) * a.prefix_ld : nullptr, a.d_table + (size_t)r * a.table_ld, units_before_own<WAY>(q.s), q.s.before, seen_by<WAY>(p, q.s, q.t)};
+}
 // A unit of a piece: its page table, its first key there, and how many keys the tile's last row sees there.
 struct Part { const int *table; int key0, seen; bool own; };
-template <int WAY> __device__ __forceinline__ Part part_at(const b200_paged_attn_args &a, const Plan &p, const Piece &q, int unit)
+template <int WAY> __device__ __forceinline__ Part part_at(const Keys &k, const Piece &q, int unit)
 {
-    constexpr int KEYS = Cut<WAY>::KEYS;
-    const int first = units_before_own<WAY>(q.s), u = q.k0 + unit, r = q.e - a.n_groups;
-    if (!q.s.own) return {a.d_prefix_table + (size_t)q.e * a.prefix_ld, u * KEYS, q.s.keys, false};
-    if (u < first) return {a.d_prefix_table + (size_t)group_of(p, r) * a.prefix_ld, u * KEYS, q.s.before, false};
-    return {a.d_table + (size_t)r * a.table_ld, (u - first) * KEYS, seen_by<WAY>(p, q.s, q.t), true};
+    const int u = q.k0 + unit;
+    if (u < k.first) return {k.prefix, u * Cut<WAY>::KEYS, k.before, false};
+    return {k.table, (u - k.first) * Cut<WAY>::KEYS, k.seen, true};
 }
 // Whether a set's rows have all of their keys in it.
 __device__ __forceinline__ bool alone(const Plan &p, const Piece &q) { return q.s.own && (q.s.before > 0 || group_of(p, q.e - p.n_groups) < 0); }
