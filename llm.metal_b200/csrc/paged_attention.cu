@@ -4,6 +4,8 @@
 #include "paged_attention_few.cuh"
 #include "paged_attention_many.cuh"
 
+#include <atomic>
+
 extern unsigned long long g_b200_launches;
 
 namespace {
@@ -43,8 +45,8 @@ template <int WAY> __device__ __forceinline__ Cuts cuts_of(const Plan &p, const 
 {
     constexpr int ROWS = Cut<WAY>::ROWS;
     const int t = i / ROWS, per_head = over(p.unit[WAY][e + 1] - p.unit[WAY][e], p.shape.by_kv);
-    const int b = p.unit[WAY][e] + h * per_head + line_before<WAY>(p, s, t) + Cut<WAY>::GAP;
-    const int w0 = quotient(b, p.per[WAY]), w1 = quotient(b + units_of<WAY>(p, s, t) - 1, p.per[WAY]);
+    const int end = p.unit[WAY][e] + h * per_head + line_before<WAY>(p, s, t + 1);           // the tile's units end where the next tile's gap begins
+    const int w0 = quotient(end - units_of<WAY>(p, s, t), p.per[WAY]), w1 = quotient(end - 1, p.per[WAY]);
     // a tile of 128 rows at most, in places for 256: two pieces in each, of every other unit
     const bool halves = WAY == 1 && s.nr - t * ROWS <= ROWS / 2;
     const long long place = (long long)(p.tile[WAY][e] + h * tiles_of<WAY>(s) + t + w0) * ROWS + i % ROWS;
@@ -72,15 +74,19 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_co
         int group = group_of(p, r);
         const Set own = set_at(p, p.n_groups + r);
         if (own.before > 0) group = -1;                      // one set
+        const Set shared = set_at(p, max(group, 0));
+        Cuts x = {}, y = {};
+#pragma unroll 1
         for (int head = first; head < first + heads; ++head) {
-            const int i = (row - p.row[r]) * G + head - h * G;
-            Cuts x = {}, y = way_of(p, own) ? cuts_of<1>(p, own, many, p.n_groups + r, h, i, HD) : cuts_of<0>(p, own, few, p.n_groups + r, h, i, HD);
-            if (group >= 0) {
-                const Set s = set_at(p, group);
-                const int j = i + (p.small[r] - p.small[p.group[group]]) * G;
-                x = way_of(p, s) ? cuts_of<1>(p, s, many, group, h, j, HD) : cuts_of<0>(p, s, few, group, h, j, HD);
-            } else if (!y.several) continue;                 // stored where it was formed
-            x.acc += lane * N; y.acc += lane * N;
+            const int i = (row - p.row[r]) * G + head - h * G, j = group >= 0 ? i + (p.small[r] - p.small[p.group[group]]) * G : 0;
+            if (head == first || !(i % FEW_ROWS) || !(j % FEW_ROWS)) {       // another tile, it may be
+                y = way_of(p, own) ? cuts_of<1>(p, own, many, p.n_groups + r, h, i, HD) : cuts_of<0>(p, own, few, p.n_groups + r, h, i, HD);
+                if (group >= 0) x = way_of(p, shared) ? cuts_of<1>(p, shared, many, group, h, j, HD) : cuts_of<0>(p, shared, few, group, h, j, HD);
+                x.acc += lane * N; y.acc += lane * N;
+            } else {
+                x.acc += HD; ++x.top; y.acc += HD; ++y.top;
+            }
+            if (group < 0 && !y.several) continue;           // stored where it was formed
             if (!waited) { pdl_wait(); waited = true; }
             const int n = x.count + y.count;
             auto top_of = [&](int j) { return j < x.count ? x.top + (long long)j * x.step : y.top + (long long)(j - x.count) * y.step; };
@@ -124,11 +130,30 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_co
     if (!waited) pdl_wait();
 }
 
+constexpr int DEVICES = 64;              // beyond these nothing is remembered
+
 int sm_count()
 {
+    static std::atomic<int> known[DEVICES];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < DEVICES && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    if (dev < DEVICES) known[dev].store(n, std::memory_order_relaxed);
     return n;
+}
+
+// Lets a kernel have all of an SM's shared memory, once a device.
+template <typename K> cudaError_t allow_all(K kern, std::atomic<unsigned long long> &done)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < DEVICES && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, kern)) != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)at.sharedSizeBytes);
+    if (e == cudaSuccess && dev < DEVICES) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
+    return e;
 }
 
 // Sizes alone: 0, or why they are refused.
@@ -154,7 +179,9 @@ Layout layout_of(const b200_paged_attn_args &a)
     Layout L = {};
     L.shape.by_g = div_of((int)G); L.shape.by_kv = div_of(a.n_kv);
     L.shape.few_most = wide ? FEW_MOST : INT_MAX; L.shape.big = wide ? BIG_ROWS : INT_MAX;
-    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 7 : 5;
+    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 11.0f : 6.7f;
+    L.shape.row_step[0] = (int)((FEW_ROWS * 256 + G - 1) / G); L.shape.row_step[1] = (int)((MANY_ROWS * 256 + G - 1) / G);
+    L.shape.each = 1;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
     const long long few_tiles = sets * ((FEW_MOST + FEW_ROWS - 1) / FEW_ROWS), full = (all + FEW_ROWS - 1) / FEW_ROWS + sets;
     const long long few_slots = (wide && few_tiles < full ? few_tiles : full) * a.n_kv + L.shape.blocks * L.shape.few_warps;
@@ -171,7 +198,7 @@ Layout layout_of(const b200_paged_attn_args &a)
 template <typename T, int HD>
 int launch(const b200_paged_attn_args &a, cudaStream_t st)
 {
-    const Layout L = layout_of(a);
+    Layout L = layout_of(a);
     if (a.work_bytes < L.bytes) return B200_E_BADARG;
     char *work = static_cast<char *>(a.d_work);
     const Pieces few = {reinterpret_cast<float *>(work + L.few_acc), reinterpret_cast<float2 *>(work + L.few_top)};
@@ -189,9 +216,13 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     }
     const size_t smem = room.plan_off + plan + 1024;
     if (smem > 227 * 1024 - 2048) return B200_E_TOOLARGE;
-    cudaError_t e = cudaFuncSetAttribute(attn_pages_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> pages_done, join_done;
+    cudaError_t e = allow_all(attn_pages_kernel<T, HD>, pages_done);
+    if (e == cudaSuccess) e = allow_all(attn_join_kernel<T, HD>, join_done);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
+    const int sets = a.n_req + a.n_groups;
+    L.shape.each = (sets + block_threads(HD) - 1) / block_threads(HD);
     cfg.gridDim = dim3((unsigned)L.shape.blocks);
     cfg.blockDim = dim3(block_threads(HD));
     cfg.dynamicSmemBytes = smem;
@@ -204,7 +235,7 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     e = cudaLaunchKernelEx(&cfg, attn_pages_kernel<T, HD>, map_k, map_v, a, L.shape, few, many, room);
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
-    if (plan > 40 * 1024 && (e = cudaFuncSetAttribute(attn_join_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan)) != cudaSuccess) return (int)e;
+    L.shape.each = (sets + JOIN_WARPS * 32 - 1) / (JOIN_WARPS * 32);
     const long long blocks = ((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS, most = (long long)JOIN_BLOCKS * L.shape.blocks;
     e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(JOIN_WARPS * 32), plan, st, a, L.shape, few, many);
     if (e != cudaSuccess) return (int)e;

@@ -56,6 +56,8 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
         const int seen = seen_by<0>(p, s, t), seen_first = s.own ? s.keys - s.rows + over(i0, by_g) + 1 : s.keys;
         const Keys keys = keys_of<0>(a, p, piece);                // (none comes before a request's own here)
         const int *table = s.own ? keys.table : keys.prefix;
+        // the first page numbers, then the queries: one round trip for both
+        int ids = lane < n ? __ldg(table + ((k0 + lane) * FEW_KEYS >> page_shift)) : 0;
         int limit[2], row_of[2], column[2];
         uint32_t q[CH / 2][4];
 #pragma unroll
@@ -73,11 +75,10 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
                 q[ks][2 + half] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 8) : 0u;
             }
         }
-        int ids = 0;
         bool outside = false;
         auto issue = [&](int i) {                            // unit k0 + i of the tile into its place of the ring
             if (i < n) {
-                if ((i & 31) == 0) {                         // page numbers, 32 units at a time
+                if ((i & 31) == 0 && i > 0) {                // page numbers, 32 units at a time
                     const int key = (k0 + i + lane) * FEW_KEYS;
                     ids = i + lane < n ? __ldg(table + (key >> page_shift)) : 0;
                 }

@@ -29,10 +29,13 @@ inline Div div_of(int d)
 
 // What the host says of a step: query heads of a key / value head, and key / value heads; sets of more than few_most query rows go the second way; a request
 // of `big` of them or more meets its prefix by itself; blocks of the kernel, and workers of the first way in one (of the second: one); what a unit
-// of the second way costs in units of the first.
+// of the second way costs in units of the first. each: sets of a thread. row_step: rows of a way's tile, in
+// 256ths, rounded up.
 struct Shape {
     Div by_g, by_kv;
-    int few_most, big, blocks, few_warps, ratio;
+    int few_most, big, blocks, few_warps, each;
+    int row_step[2];
+    float ratio;
 };
 
 // Where a way's pieces lie in d_work: [slot][rows of a tile][hd] sums and [slot][rows of a tile] (largest score, sum), scores in units of log 2. A tile's piece of
@@ -41,9 +44,9 @@ struct Pieces { float *acc; float2 *top; };
 
 namespace {
 
-// The two ways: rows of a tile, keys of a unit, fewest units of a worker, units' worth of a gap.
+// The two ways: rows of a tile, keys of a unit, fewest units of a worker, units' worth of a gap (two at least: see line_before).
 template <int WAY> struct Cut;
-template <> struct Cut<0> { static constexpr int ROWS = 16, KEYS = 16, LEAST = 4, GAP = 1; };
+template <> struct Cut<0> { static constexpr int ROWS = 16, KEYS = 16, LEAST = 4, GAP = 2; };
 template <> struct Cut<1> { static constexpr int ROWS = 256, KEYS = 64, LEAST = 4, GAP = 6; };
 
 // What a block knows of the step, in shared memory.
@@ -63,7 +66,7 @@ __host__ __device__ inline size_t plan_bytes(int n_req, int n_groups)
 }
 
 __device__ __forceinline__ int over(int n, const Div &d) { return (int)((__umulhi((unsigned)n, d.m) + (unsigned)n) >> d.s); }
-// n / d for quotients below 2^20 or so
+// n / d, where the quotient is below 2^22
 __device__ __forceinline__ int quotient(int n, int d)
 {
     int q = (int)__fdividef((float)n, (float)d);
@@ -132,130 +135,128 @@ template <int WAY> __device__ __forceinline__ int units_of(const Plan &p, const 
 {
     return units_before_own<WAY>(s) + (seen_by<WAY>(p, s, t) + Cut<WAY>::KEYS - 1) / Cut<WAY>::KEYS;
 }
-// where the t-th tile of a head begins on the line, its gap included
+// Where the t-th tile of a head begins on the line, its gap included. A request's tiles see about row_step / 256 keys more from one to the next: their places come
+// from the sum of that progression, with one unit more a tile for what rounding takes, and a tile's gap is what its units leave (GAP - 2 at least).
 template <int WAY> __device__ __forceinline__ int line_before(const Plan &p, const Set &s, int t)
 {
-    if (!s.own) return t * (Cut<WAY>::GAP + units_of<WAY>(p, s, 0));
-    int n = t * Cut<WAY>::GAP;
-#pragma unroll 1
-    for (int i = 0; i < t; ++i) n += units_of<WAY>(p, s, i);
-    return n;
+    constexpr int GAP = Cut<WAY>::GAP, KEYS = Cut<WAY>::KEYS;
+    if (!s.own) return t * (GAP + units_of<WAY>(p, s, 0));
+    const long long keys = (long long)(s.keys - s.rows) * t + (((long long)p.shape.row_step[WAY] * t * (t + 1)) >> 9);
+    return t * (GAP + 1 + units_before_own<WAY>(s)) + (int)(keys / KEYS);
 }
 
 // Units of a worker: equal stretches, and none so short that joining costs more than it spreads.
-template <int WAY> __device__ __forceinline__ int stretch(int units, int workers) { return max(Cut<WAY>::LEAST, (int)(((unsigned)units + workers - 1) / (unsigned)workers)); }
+template <int WAY> __device__ __forceinline__ int stretch(int units, int workers)
+{
+    return max(Cut<WAY>::LEAST, (int)(((unsigned)units + workers - 1) / (unsigned)workers));
+}
 
 // Reads the lengths and lays the lines; false (for the whole block) if something does not fit. `mem` holds plan_bytes; for blocks of up to 16 warps.
-__device__ __noinline__ bool make_plan(const b200_paged_attn_args &a, const Shape &shape, char *mem, Plan &plan)
+// This runs at the head of every launch, from cold instruction caches, where 8 instructions come in about 125 clocks: short code counts, so loops stay loops.
+__device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const Shape &shape, char *mem, Plan &plan)
 {
     __shared__ int4 red[16];
-    __shared__ float red_f[16];
-    __shared__ int red_s[16];
-    const int sets = a.n_req + a.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    __shared__ float2 red_f[16];
+    const int sets = a.n_req + a.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int *const unit = reinterpret_cast<int *>(mem), *const row = unit + 4 * (sets + 1), *const group = row + 3 * a.n_req + 2;
     if (threadIdx.x == 0) {
         plan.n_req = a.n_req; plan.n_groups = a.n_groups; plan.shape = shape;
-        int *at = reinterpret_cast<int *>(mem);
-        for (int w = 0; w < 2; ++w) { plan.unit[w] = at; plan.tile[w] = at + sets + 1; at += 2 * (sets + 1); }
-        plan.row = at; plan.len = at + a.n_req + 1; plan.small = at + 2 * a.n_req + 1;
-        plan.group = at + 3 * a.n_req + 2; plan.prefix = plan.group + a.n_groups + 1;
+        plan.unit[0] = unit; plan.tile[0] = unit + sets + 1; plan.unit[1] = unit + 2 * (sets + 1); plan.tile[1] = unit + 3 * (sets + 1);
+        plan.row = plan.small = row; plan.len = row + a.n_req + 1;
+        plan.group = group; plan.prefix = group + a.n_groups + 1;
     }
-    __syncthreads();
-    Plan p = plan;
+    int bad = 0, big = 0;
 #pragma unroll 1
-    for (int i = threadIdx.x; i <= max(a.n_req, a.n_groups); i += blockDim.x) {
-        int row = 0, len = 0, group = 0, prefix = 0;         // all loads on their way before the first one is stored
-        if (i <= a.n_req) row = a.d_row_start[i];
-        if (i < a.n_req) len = a.d_len[i];
-        if (a.n_groups && i <= a.n_groups) group = a.d_group_start[i];
-        if (i < a.n_groups) prefix = a.d_prefix_len[i];
-        if (i <= a.n_req) p.row[i] = row;
-        if (i < a.n_req) p.len[i] = len;
-        if (a.n_groups && i <= a.n_groups) p.group[i] = group;
-        if (i < a.n_groups) p.prefix[i] = prefix;
+    for (int i = threadIdx.x; i <= a.n_req; i += blockDim.x) {           // (n_groups <= n_req)
+        const bool is_req = i < a.n_req, is_group = i < a.n_groups;
+        const int r0 = a.d_row_start[i], r1 = is_req ? a.d_row_start[i + 1] : r0, len = is_req ? a.d_len[i] : 0;
+        const int g0 = i <= a.n_groups && a.n_groups ? a.d_group_start[i] : 0, g1 = is_group ? a.d_group_start[i + 1] : g0, prefix = is_group ? a.d_prefix_len[i] : 0;
+        row[i] = r0;
+        if (is_req) row[a.n_req + 1 + i] = len;
+        if (i <= a.n_groups) group[i] = g0;
+        if (is_group) group[a.n_groups + 1 + i] = prefix;
+        bad |= (i == 0 && r0 != 0) || r1 < r0 || r1 > a.max_rows || (r1 > r0 && (len < r1 - r0 || len > a.table_ld * a.page));
+        bad |= g0 < 0 || g1 < g0 || g1 > a.n_req || prefix < 0 || prefix > a.prefix_ld * a.page;
+        big |= !bad && (r1 - r0) * shape.by_g.d >= shape.big;
     }
-    __syncthreads();
-    int bad = 0, any_big = 0;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < a.n_req; i += blockDim.x) {
-        const int r0 = p.row[i], r1 = p.row[i + 1], len = p.len[i];
-        bad |= (i == 0 && r0 != 0) || r1 < r0 || r1 > a.max_rows;
-        bad |= r1 > r0 && (len < r1 - r0 || len > (long long)a.table_ld * a.page);
-        any_big |= !bad && (r1 - r0) * shape.by_g.d >= shape.big;
-    }
-#pragma unroll 1
-    for (int i = threadIdx.x; i < a.n_groups; i += blockDim.x) {
-        const int g0 = p.group[i], g1 = p.group[i + 1];
-        bad |= g0 < 0 || g1 < g0 || g1 > a.n_req || p.prefix[i] < 0 || p.prefix[i] > (long long)a.prefix_ld * a.page;
-    }
-    bad = __syncthreads_or(bad);
-    if (bad) {
-        if (blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
-        return false;
-    }
-    any_big = a.n_groups ? __syncthreads_or(any_big) : 0;
-    if (!any_big) {
-        p.small = p.row;                                     // no row meets a prefix by itself
-        if (threadIdx.x == 0) plan.small = p.row;
-    } else {
-        const int each = (a.n_req + blockDim.x - 1) / blockDim.x, r0 = min(a.n_req, (int)threadIdx.x * each), r1 = min(a.n_req, r0 + each);
-        auto rows = [&](int r) { const int n = p.row[r + 1] - p.row[r]; return n * shape.by_g.d >= shape.big && group_of(p, r) >= 0 ? 0 : n; };
-        int n = 0;
-        for (int r = r0; r < r1; ++r) n += rows(r);
-        int in = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, in, o);
-            if (lane >= o) in += x;
+    if (__syncthreads_or(bad | big)) {
+        bad = __syncthreads_or(bad);
+        if (bad) {
+            if (blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
+            return false;
         }
-        if (lane == 31) red_s[warp] = in;
-        __syncthreads();
-        in -= n;
-        for (int w = 0; w < warp; ++w) in += red_s[w];
-        for (int r = r0; r < r1; ++r) {
-            p.small[r] = in;
-            in += rows(r);
-            if (r == a.n_req - 1) p.small[a.n_req] = in;
+        if (a.n_groups) {                                    // rows that are not big ones, 32 requests at a time
+            int *const small = row + 2 * a.n_req + 1;
+            if (warp == 0) {
+                int before = 0;
+#pragma unroll 1
+                for (int r = lane; r - lane < a.n_req; r += 32) {
+                    const int rows = r < a.n_req ? row[r + 1] - row[r] : 0, mine = rows * shape.by_g.d >= shape.big && group_of(plan, r) >= 0 ? 0 : rows;
+                    int in = mine;
+#pragma unroll 1
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int x = __shfl_up_sync(0xffffffffu, in, o);
+                        if (lane >= o) in += x;
+                    }
+                    if (r <= a.n_req) small[r] = before + in - mine;
+                    before += __shfl_sync(0xffffffffu, in, 31);
+                }
+                if (lane == 0) { small[a.n_req] = before; plan.small = small; }
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
     // the two lines: (units, tiles) of each, for the sets of this thread, of the warp, of the block
-    const int each = (sets + blockDim.x - 1) / blockDim.x, e0 = min(sets, (int)threadIdx.x * each), e1 = min(sets, e0 + each);
+    const int e0 = min(sets, (int)threadIdx.x * shape.each), e1 = min(sets, e0 + shape.each);
     int4 mine = make_int4(0, 0, 0, 0);
-    float size = 0.0f;
+    float size = 0.0f, many_cost = 0.0f;
 #pragma unroll 1
     for (int e = e0; e < e1; ++e) {
-        const Set s = set_at(p, e);
+        const Set s = set_at(plan, e);
         int n = 0, k = 0;
-        const int way = way_of(p, s);
+        const int way = way_of(plan, s);
         if (s.nr > 0 && s.keys > 0) {
-            k = way ? tiles_of<1>(s) : tiles_of<0>(s);
-            n = way ? line_before<1>(p, s, k) : line_before<0>(p, s, k);
+            float cost;
+            if (way) {
+                k = tiles_of<1>(s);
+                n = line_before<1>(plan, s, k);
+                // a tile whose rows fit into one stream costs half
+                const int last = s.nr - (k - 1) * Cut<1>::ROWS;
+                cost = (float)n * shape.ratio * (last > Cut<1>::ROWS / 2 ? 1.0f : 1.0f - __fdividef(0.5f, (float)k));
+            } else {
+                k = tiles_of<0>(s);
+                n = line_before<0>(plan, s, k);
+                cost = (float)n;
+            }
             size += (float)n * (float)shape.by_kv.d;
+            if (way) many_cost += cost * (float)shape.by_kv.d;
             n *= shape.by_kv.d; k *= shape.by_kv.d;
         }
-        p.unit[0][e] = way ? 0 : n; p.tile[0][e] = way ? 0 : k;          // summed up below, by the same thread
-        p.unit[1][e] = way ? n : 0; p.tile[1][e] = way ? k : 0;
+        int *const at = unit + e + way * 2 * (sets + 1);     // summed up below, by the same thread
+        at[0] = n; at[sets + 1] = k;
+        int *const other = unit + e + (way ^ 1) * 2 * (sets + 1);
+        other[0] = 0; other[sets + 1] = 0;
         if (way) { mine.z += n; mine.w += k; } else { mine.x += n; mine.y += k; }
     }
     int4 in = mine;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, in.x, o), y = __shfl_up_sync(0xffffffffu, in.y, o);
         const int z = __shfl_up_sync(0xffffffffu, in.z, o), w = __shfl_up_sync(0xffffffffu, in.w, o);
-        if (lane >= o) { in.x += x; in.y += y; in.z += z; in.w += w; }
+        const float f = __shfl_up_sync(0xffffffffu, size, o), g = __shfl_up_sync(0xffffffffu, many_cost, o);
+        if (lane >= o) { in.x += x; in.y += y; in.z += z; in.w += w; size += f; many_cost += g; }
     }
-    size = warp_sum(size);
-    if (lane == 31) { red[warp] = in; red_f[warp] = size; }
+    if (lane == 31) { red[warp] = in; red_f[warp] = make_float2(size, many_cost); }
     __syncthreads();
     int4 all = make_int4(0, 0, 0, 0);
     in.x -= mine.x; in.y -= mine.y; in.z -= mine.z; in.w -= mine.w;
-    size = 0.0f;
+    size = many_cost = 0.0f;
 #pragma unroll 1
-    for (int w = 0; w < nw; ++w) {
+    for (int w = 0; w * 32 * shape.each < sets; ++w) {       // (the others have none)
         const int4 x = red[w];
-        if (w == warp) { in.x += all.x; in.y += all.y; in.z += all.z; in.w += all.w; }
+        if (w < warp) { in.x += x.x; in.y += x.y; in.z += x.z; in.w += x.w; }
         all.x += x.x; all.y += x.y; all.z += x.z; all.w += x.w;
-        size += red_f[w];
+        size += red_f[w].x; many_cost += red_f[w].y;
     }
     if (size > 2.0e9f) {                                     // lines of 2^31 units: tens of terabytes of keys
         if (blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
@@ -263,17 +264,18 @@ __device__ __noinline__ bool make_plan(const b200_paged_attn_args &a, const Shap
     }
 #pragma unroll 1
     for (int e = e0; e < e1; ++e) {
-        const int x = p.unit[0][e], y = p.tile[0][e], z = p.unit[1][e], w = p.tile[1][e];
-        p.unit[0][e] = in.x; p.tile[0][e] = in.y; p.unit[1][e] = in.z; p.tile[1][e] = in.w;
+        int *const at = unit + e;
+        const int x = at[0], y = at[sets + 1], z = at[2 * (sets + 1)], w = at[3 * (sets + 1)];
+        at[0] = in.x; at[sets + 1] = in.y; at[2 * (sets + 1)] = in.z; at[3 * (sets + 1)] = in.w;
         in.x += x; in.y += y; in.z += z; in.w += w;
     }
     if (threadIdx.x == 0) {
-        p.unit[0][sets] = all.x; p.tile[0][sets] = all.y; p.unit[1][sets] = all.z; p.tile[1][sets] = all.w;
+        unit[sets] = all.x; unit[2 * sets + 1] = all.y; unit[3 * sets + 2] = all.z; unit[4 * sets + 3] = all.w;
         // blocks for each way: by their shares of the work, no more than have units to begin with, one at least
         int many = 0;
         if (all.z > 0) {
-            const float a1 = (float)all.z * (float)shape.ratio, a0 = (float)all.x;
-            many = all.x == 0 ? shape.blocks : max(1, min(shape.blocks - 1, (int)((float)shape.blocks * a1 / (a0 + a1) + 0.5f)));
+            const float a1 = many_cost, a0 = (float)all.x;
+            many = all.x == 0 ? shape.blocks : max(1, min(shape.blocks - 1, (int)((float)shape.blocks * __fdividef(a1, a0 + a1) + 0.5f)));
             many = min(many, (all.z + Cut<1>::LEAST - 1) / Cut<1>::LEAST);
         }
         plan.many_blocks = many;
@@ -301,7 +303,6 @@ template <int WAY> struct Walk {
     }
     __device__ __forceinline__ bool next(const Plan &p, Piece &q)
     {
-        constexpr int GAP = Cut<WAY>::GAP;
         while (at < end) {
             const int *unit = p.unit[WAY];
             while (unit[e + 1] <= at) ++e;
@@ -310,14 +311,24 @@ template <int WAY> struct Walk {
             q.tiles = tiles_of<WAY>(q.s);
             const int head = over(unit[e + 1] - unit[e], p.shape.by_kv);
             q.h = quotient(at - unit[e], head);
-            int rest = at - unit[e] - q.h * head;
+            int rest = at - unit[e] - q.h * head, end_of = head;
             q.t = 0;
-            q.ut = units_of<WAY>(p, q.s, 0);
-            while (rest >= GAP + q.ut) { rest -= GAP + q.ut; q.ut = units_of<WAY>(p, q.s, ++q.t); }
-            const int n = min(GAP + q.ut - rest, end - at);
+            if (q.tiles > 1) {                               // the last tile that begins at or before the place
+                int hi = q.tiles;
+#pragma unroll 1
+                while (hi - q.t > 1) {
+                    const int mid = (q.t + hi) >> 1;
+                    if (line_before<WAY>(p, q.s, mid) <= rest) q.t = mid; else hi = mid;
+                }
+                const int begin = line_before<WAY>(p, q.s, q.t);
+                rest -= begin;
+                end_of = line_before<WAY>(p, q.s, q.t + 1) - begin;
+            }
+            q.ut = units_of<WAY>(p, q.s, q.t);
+            const int gap = end_of - q.ut, n = min(end_of - rest, end - at);
             at += n;
-            q.k0 = max(0, rest - GAP);
-            q.n = rest + n - GAP - q.k0;
+            q.k0 = max(0, rest - gap);
+            q.n = rest + n - gap - q.k0;
             if (q.n > 0) return true;                        // (not only a gap)
         }
         return false;
