@@ -10,7 +10,7 @@ extern unsigned long long g_b200_launches;
 
 namespace {
 
-constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 8;
+constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 4;
 // Sets of more query rows than FEW_MOST go the second way, where hd is one of its own; a request of BIG_ROWS of them fills a stream there by itself.
 constexpr int FEW_MOST = 16, BIG_ROWS = 128;
 
@@ -91,11 +91,7 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_co
             const int n = x.count + y.count;
             auto top_of = [&](int j) { return j < x.count ? x.top + (long long)j * x.step : y.top + (long long)(j - x.count) * y.step; };
             auto acc_of = [&](int j) { return j < x.count ? x.acc + (long long)j * x.step * HD : y.acc + (long long)(j - x.count) * y.step * HD; };
-            float top = -INFINITY;
-            for (int j = lane; j < n; j += 32) top = fmaxf(top, top_of(j)->x);
-            top = warp_max(top);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float l = 0.0f, o[N];
+            float top = -INFINITY, l = 0.0f, o[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) o[k] = 0.0f;
 #pragma unroll 1
@@ -112,6 +108,14 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_co
                         for (int q = 0; q < N; q += 4) *reinterpret_cast<float4 *>(&v[j][q]) = *reinterpret_cast<const float4 *>(from + q);
                     } else *reinterpret_cast<float2 *>(v[j]) = *reinterpret_cast<const float2 *>(from);
                 }
+                float higher = top;
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) higher = fmaxf(higher, ml[j].x);
+                const float base = higher == -INFINITY ? 0.0f : higher, down = ex2(top - base);
+                top = higher;
+                l *= down;
+#pragma unroll
+                for (int q = 0; q < N; ++q) o[q] *= down;
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const bool on = j0 + j < n;
