@@ -408,7 +408,10 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
             // ---- pages into the ring ----
-            const int box = min(a.page, MANY_KEYS), page_shift = 31 - __clz(a.page), boxes = MANY_KEYS / box;
+            // A copy takes up to 64 tokens of a page by 64 numbers; a lane to each. A unit's page numbers are asked for one unit ahead, once for its keys and once for its
+            // values: with that round trip in each step the ring would fill at half of its rate.
+            const int page_shift = 31 - __clz(a.page), box_shift = min(page_shift, 6), box = 1 << box_shift;
+            const int mine = lane / NB, part = lane % NB;
             asm volatile("fence.proxy.async;" ::: "memory");     // rows that an earlier kernel stored, read by the copy engine
             Place at = {0, 0};
             bool outside = false, ok = true;
@@ -416,29 +419,37 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             Piece piece;
             while (ok && walk.next(p, piece)) {
                 const Streams w = streams_of(p, piece);
-                const int n = piece.n;
+                const int n = piece.n, lead = w.lead;
                 const Keys keys = keys_of<1>(a, p, piece);
-                auto load = [&](int unit, bool values) {         // by the whole warp
-                    const int slot = at.slot;
-                    const uint32_t phase = at.phase;
-                    at.next(slots);
+                struct Unit { int there, y, id; };               // copies, the first token in the page, this lane's page
+                auto unit_at = [&](int unit) {
                     const Part u = part_at<1>(keys, piece, unit);
-                    const int there = min(boxes, (u.seen - u.key0 + box - 1) / box);
-                    const int mine = lane / NB, part = lane % NB, key = u.key0 + mine * box;
-                    int id = mine < there ? __ldg(u.table + (key >> page_shift)) : 0;
-                    if (id < 0 || id >= a.n_pages) { outside = true; id = -1; }
-                    if (!__all_sync(0xffffffffu, wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag))) { ok = false; return; }
-                    if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)there * box * 128 * NB);
-                    __syncwarp();
-                    if (mine < there)                            // an id of -1 is outside the map and reads as zeros
-                        tma_load_3d(ring + slot * SLOT + part * KEY64 + mine * box * 128, values ? &map_v : &map_k, part * 64, key & (a.page - 1),
-                                    id < 0 ? -1 : id * a.n_kv + piece.h, &full_bar[slot]);
+                    Unit x;
+                    x.there = min(MANY_KEYS >> box_shift, (u.seen - u.key0 + box - 1) >> box_shift);
+                    const int key = u.key0 + (mine << box_shift);
+                    x.y = key & (a.page - 1);
+                    x.id = mine < x.there ? __ldg(u.table + (key >> page_shift)) : 0;
+                    return x;
                 };
-                    for (int j = 0; j < w.lead && ok; ++j) load(j, false);
-                    for (int j = 0; j < n && ok; ++j) {
-                        load(j, true);
-                        if (ok && j + w.lead < n) load(j + w.lead, false);
-                    }
+                Unit next[2] = {unit_at(0), unit_at(0)};
+                auto load = [&](int unit, int values) {          // by the whole warp
+                    const Unit u = values ? next[1] : next[0];
+                    if (unit + 1 < n) { if (values) next[1] = unit_at(unit + 1); else next[0] = unit_at(unit + 1); }
+                    const bool there = u.id >= 0 && u.id < a.n_pages;
+                    outside |= !there;
+                    if (!__all_sync(0xffffffffu, wait_or_abort(&empty_bar[at.slot], at.phase ^ 1, abort_flag))) { ok = false; return; }
+                    if (lane == 0) mbar_expect_tx(&full_bar[at.slot], (uint32_t)u.there << box_shift << 7 << (NB - 1));
+                    __syncwarp();
+                    if (mine < u.there)                          // a page of -1 is outside the map and reads as zeros
+                        tma_load_3d(ring + at.slot * SLOT + part * KEY64 + (mine << box_shift << 7), values ? &map_v : &map_k, part * 64, u.y, there ? u.id * a.n_kv + piece.h : -1,
+                                    &full_bar[at.slot]);
+                    at.next(slots);
+                };
+#pragma unroll 1
+                for (int j = -lead; j < n && ok; ++j) {          // keys `lead` units ahead of values
+                    if (j >= 0) load(j, 1);
+                    if (ok && j + lead < n) load(j + lead, 0);
+                }
             }
             if (!ok) give_up();
             if (outside && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
