@@ -183,7 +183,7 @@ Layout layout_of(const b200_paged_attn_args &a)
     Layout L = {};
     L.shape.by_g = div_of((int)G); L.shape.by_kv = div_of(a.n_kv);
     L.shape.few_most = wide ? FEW_MOST : INT_MAX; L.shape.big = wide ? BIG_ROWS : INT_MAX;
-    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 11.0f : 6.7f;
+    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;
     L.shape.row_step[0] = (int)((FEW_ROWS * 256 + G - 1) / G); L.shape.row_step[1] = (int)((MANY_ROWS * 256 + G - 1) / G);
     L.shape.each = 1;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker

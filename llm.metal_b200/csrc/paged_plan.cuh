@@ -220,9 +220,9 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
             if (way) {
                 k = tiles_of<1>(s);
                 n = line_before<1>(plan, s, k);
-                // a tile whose rows fit into one stream costs four fifths
+                // a tile whose rows fit into one stream costs two thirds
                 const int last = s.nr - (k - 1) * Cut<1>::ROWS;
-                cost = (float)n * shape.ratio * (last > Cut<1>::ROWS / 2 ? 1.0f : 1.0f - __fdividef(0.2f, (float)k));
+                cost = (float)n * shape.ratio * (last > Cut<1>::ROWS / 2 ? 1.0f : 1.0f - __fdividef(0.35f, (float)k));
             } else {
                 k = tiles_of<0>(s);
                 n = line_before<0>(plan, s, k);
