@@ -105,22 +105,49 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
         }
     }
     if (why) return;
-    const int first = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+    // Four at a time: one search, one round trip to the table and the stack, and 16-byte stores where the arrays are aligned for them.
+    const int first = 4 * (blockIdx.x * blockDim.x + threadIdx.x), step = 4 * gridDim.x * blockDim.x, shift = 31 - __clz(a.page);
+#pragma unroll 1
     for (int p = first; p < total.y; p += step) {
-        const int q = owner_of(s_page, n, p);
-        if (RELEASE) a.d_free[free_n + p] = a.d_table[(size_t)q * a.table_ld + (p - s_page[q])];
-        else a.d_table[(size_t)q * a.table_ld + (s_len[q] + a.page - 1) / a.page + (p - s_page[q])] = a.d_free[free_n - 1 - p];
+        int q = owner_of(s_page, n, p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (p + k >= total.y) break;
+            while (q + 1 < n && s_page[q + 1] <= p + k) ++q;
+            if (RELEASE) a.d_free[free_n + p + k] = a.d_table[(size_t)q * a.table_ld + (p + k - s_page[q])];
+            else a.d_table[(size_t)q * a.table_ld + ((s_len[q] + a.page - 1) >> shift) + (p + k - s_page[q])] = a.d_free[free_n - 1 - p - k];
+        }
     }
     if (RELEASE) return;
     unsigned outside = 0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.d_slot) | reinterpret_cast<uintptr_t>(a.d_pos)) & 15) == 0;
+#pragma unroll 1
     for (int m = first; m < total.x; m += step) {
-        const int q = owner_of(s_row, n, m), token = s_len[q] + (m - s_row[q]), k = token / a.page, held = (s_len[q] + a.page - 1) / a.page;
-        // the pages of this call come from the stack: their numbers in the table may not be there yet
-        const int id = k < held ? a.d_table[(size_t)q * a.table_ld + k] : a.d_free[free_n - 1 - (s_page[q] + k - held)];
-        const bool ok = id >= 0 && id < a.n_pages;
-        a.d_slot[m] = ok ? id * a.page + token % a.page : -1;
-        a.d_pos[m] = (a.d_base ? a.d_base[q] : 0) + token;
-        if (!ok) outside = B200_PAGED_BAD_PAGE;
+        int q = owner_of(s_row, n, m), slot[4], pos[4], token_in_page[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at_row = min(m + k, total.x - 1);
+            while (q + 1 < n && s_row[q + 1] <= at_row) ++q;
+            const int token = s_len[q] + (at_row - s_row[q]), page = token >> shift, held = (s_len[q] + a.page - 1) >> shift;
+            // the pages of this call come from the stack: their numbers in the table may not be there yet
+            slot[k] = page < held ? a.d_table[(size_t)q * a.table_ld + page] : a.d_free[free_n - 1 - (s_page[q] + page - held)];
+            pos[k] = (a.d_base ? a.d_base[q] : 0) + token;
+            token_in_page[k] = token & (a.page - 1);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool ok = slot[k] >= 0 && slot[k] < a.n_pages;
+            slot[k] = ok ? (slot[k] << shift) + token_in_page[k] : -1;
+            if (!ok) outside = B200_PAGED_BAD_PAGE;
+        }
+        if (wide && m + 4 <= total.x) {
+            *reinterpret_cast<int4 *>(a.d_slot + m) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4 *>(a.d_pos + m) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (m + k < total.x) { a.d_slot[m + k] = slot[k]; a.d_pos[m + k] = pos[k]; }
+        }
     }
     report(a.d_status, outside);
 }
@@ -178,7 +205,7 @@ template <> struct Vec<1> { using F = float; using H = uint16_t; };
 template <> struct Vec<2> { using F = float2; using H = uint32_t; };
 template <> struct Vec<4> { using F = float4; using H = uint2; };
 
-constexpr int STORE_WARPS = 8;
+constexpr int STORE_WARPS = 8, STORE_AHEAD = 4;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __grid_constant__ b200_paged_store_args a, int heads_per_block)
@@ -197,57 +224,75 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __g
     }
     const float freq = a.d_inv_freq && threadIdx.x < HALF ? a.d_inv_freq[threadIdx.x] : 0.0f;
     pdl_wait();
-    if (m >= *a.d_rows) return;
-    if (threadIdx.x < HALF) {
-        constexpr double TURN = 6.283185307179586476925;
-        const double t = (double)a.d_pos[m] * (double)freq;
+    // all loads at once, the count's among them: rows up to max_rows exist, and what lies behind the last one is only not stored
+    const int rows = *a.d_rows, slot = a.d_slot[m], pos = a.d_pos[m];
+    const int heads = a.n_q + 2 * a.n_kv, h1 = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
+    const float *row = a.d_qkv + (long long)m * a.qkv_ld;
+    float x[STORE_AHEAD][2 * N];                             // heads on their way: the first ones under the angles
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int k = 0; k < STORE_AHEAD; ++k) {
+            const int h = h0 + k * STORE_WARPS;
+            if (h < h1) {
+                *reinterpret_cast<F *>(x[k]) = *reinterpret_cast<const F *>(row + h * HD + d);
+                *reinterpret_cast<F *>(x[k] + N) = *reinterpret_cast<const F *>(row + h * HD + HALF + d);
+            }
+        }
+    };
+    int h0 = blockIdx.y * heads_per_block + warp;
+    load(h0);
+    if (m >= rows) return;
+    if (threadIdx.x < HALF && a.d_inv_freq) {
+        constexpr double TURN = 6.283185307179586476925, PER_TURN = 0.15915494309189533577;
+        const double t = (double)pos * (double)freq;
         float sn, cs;
-        sincosf((float)(t - rint(t / TURN) * TURN), &sn, &cs);
+        sincosf((float)(t - rint(t * PER_TURN) * TURN), &sn, &cs);
         s_cos[threadIdx.x] = cs; s_sin[threadIdx.x] = sn;
     }
-    const int slot = a.d_slot[m];
     const bool in_pool = slot >= 0 && slot < a.n_pages * a.page;
     if (!in_pool && threadIdx.x == 0 && blockIdx.y == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
     __syncthreads();
-    const int heads = a.n_q + 2 * a.n_kv, h1 = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
-    const float *row = a.d_qkv + (long long)m * a.qkv_ld;
-#pragma unroll 2
-    for (int h = blockIdx.y * heads_per_block + warp; h < h1; h += STORE_WARPS) {
-        float x[2 * N];
-        *reinterpret_cast<F *>(x) = *reinterpret_cast<const F *>(row + h * HD + d);
-        *reinterpret_cast<F *>(x + N) = *reinterpret_cast<const F *>(row + h * HD + HALF + d);
-        if (h < a.n_q + a.n_kv) {
-            const bool is_q = h < a.n_q;
-            if (is_q ? a.d_q_gamma != nullptr : a.d_k_gamma != nullptr) {
-                float ss = 0.0f;
+    const int shift = 31 - __clz(a.page);
+    const long long at = ((long long)(slot >> shift) * a.n_kv << shift) + (slot & (a.page - 1));       // of head 0: heads are a page apart
+    for (; h0 < h1; h0 += STORE_AHEAD * STORE_WARPS) {
 #pragma unroll
-                for (int j = 0; j < 2 * N; ++j) ss = fmaf(x[j], x[j], ss);
-                const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.eps);
+        for (int k = 0; k < STORE_AHEAD; ++k) {
+            const int h = h0 + k * STORE_WARPS;
+            if (h >= h1) break;
+            if (h < a.n_q + a.n_kv) {
+                const bool is_q = h < a.n_q;
+                if (is_q ? a.d_q_gamma != nullptr : a.d_k_gamma != nullptr) {
+                    float ss = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 2 * N; ++j) x[j] *= (is_q ? gq[j] : gk[j]) * inv;
-            }
-            if (a.d_inv_freq) {
+                    for (int j = 0; j < 2 * N; ++j) ss = fmaf(x[k][j], x[k][j], ss);
+                    const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.eps);
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float cs = s_cos[d + j], sn = s_sin[d + j], lo = x[j], hi = x[N + j];
-                    x[j] = lo * cs - hi * sn; x[N + j] = lo * sn + hi * cs;
+                    for (int j = 0; j < 2 * N; ++j) x[k][j] *= (is_q ? gq[j] : gk[j]) * inv;
+                }
+                if (a.d_inv_freq) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const float cs = s_cos[d + j], sn = s_sin[d + j], lo = x[k][j], hi = x[k][N + j];
+                        x[k][j] = lo * cs - hi * sn; x[k][N + j] = lo * sn + hi * cs;
+                    }
                 }
             }
-        }
-        uint16_t b[2 * N];
+            uint16_t b[2 * N];
 #pragma unroll
-        for (int j = 0; j < 2 * N; ++j) b[j] = to_bits<T>(x[j]);
-        uint16_t *to;
-        if (h < a.n_q) to = static_cast<uint16_t *>(a.d_q) + (long long)m * a.q_ld + h * HD;
-        else {
-            const int kv = (h - a.n_q) % a.n_kv;
-            if (!in_pool) continue;
-            to = static_cast<uint16_t *>(h < a.n_q + a.n_kv ? a.d_k_pool : a.d_v_pool) + (((long long)(slot / a.page) * a.n_kv + kv) * a.page + slot % a.page) * HD;
+            for (int j = 0; j < 2 * N; ++j) b[j] = to_bits<T>(x[k][j]);
+            uint16_t *to;
+            if (h < a.n_q) to = static_cast<uint16_t *>(a.d_q) + (long long)m * a.q_ld + h * HD;
+            else {
+                const bool is_k = h < a.n_q + a.n_kv;
+                if (!in_pool) continue;
+                to = static_cast<uint16_t *>(is_k ? a.d_k_pool : a.d_v_pool) + (at + ((long long)(h - a.n_q - (is_k ? 0 : a.n_kv)) << shift)) * HD;
+            }
+            H w[2];
+            memcpy(w, b, sizeof(w));
+            *reinterpret_cast<H *>(to + d) = w[0];
+            *reinterpret_cast<H *>(to + HALF + d) = w[1];
         }
-        H w[2];
-        memcpy(w, b, sizeof(w));
-        *reinterpret_cast<H *>(to + d) = w[0];
-        *reinterpret_cast<H *>(to + HALF + d) = w[1];
+        if (h0 + STORE_AHEAD * STORE_WARPS < h1) load(h0 + STORE_AHEAD * STORE_WARPS);
     }
 }
 
