@@ -190,8 +190,9 @@ int launch_pages(const b200_pages_args *ap, void *stream)
 }
 
 // ---- new rows into their slots ------------------------------------------------------------------------------------------------
-// Bound by memory: 4 bytes read and 2 written a number. A warp takes a head at a time; its lanes hold the pairs (d, d + hd / 2), so that the norm is a
-// shuffle and the rotation stays in the lane. The angle pos * inv_freq is formed in 64 bits (exact) and brought into one turn before the
+// Bound by memory: 4 bytes read and 2 written a number. hd / 8 lanes hold a head, each four numbers of its lower half and the four that they turn with, so that
+// the norm is a shuffle or two and the rotation stays in the lane. (A warp to a head of 128, four numbers a lane, took 140 instructions a head, and
+// 8191 rows of 32 heads 50 us.) The angle pos * inv_freq is formed in 64 bits (exact) and brought into one turn before the
 // 32-bit sine and cosine: as a 32-bit product it is off by pos * 2^-24, more than binary16's step from position 8000 on. One a lane pair and
 // block. q, k and v are rounded once, to the type of the cache that the tensor cores read.
 template <typename T> __device__ __forceinline__ uint16_t to_bits(float x)
@@ -200,46 +201,44 @@ template <typename T> __device__ __forceinline__ uint16_t to_bits(float x)
     else return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
 
-template <int N> struct Vec;
-template <> struct Vec<1> { using F = float; using H = uint16_t; };
-template <> struct Vec<2> { using F = float2; using H = uint32_t; };
-template <> struct Vec<4> { using F = float4; using H = uint2; };
-
-constexpr int STORE_WARPS = 8, STORE_AHEAD = 4;
+constexpr int STORE_WARPS = 8, STORE_AHEAD = 2;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __grid_constant__ b200_paged_store_args a, int heads_per_block)
 {
-    constexpr int HALF = HD / 2, N = HALF / 32;              // pairs of a lane
-    using F = typename Vec<N>::F;
-    using H = typename Vec<N>::H;
-    __shared__ float s_cos[HALF], s_sin[HALF];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = blockIdx.x, d = lane * N;
+    constexpr int HALF = HD / 2, N = 4, LANES = HD / 8, HEADS = 32 / LANES, STEP = STORE_WARPS * HEADS;        // lanes of a head, heads of a warp, of a round
+    __shared__ __align__(16) float s_cos[HALF], s_sin[HALF];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LANES * N;
+    const int m = blockIdx.x;
     pdl_launch_dependents();
     float gq[2 * N], gk[2 * N];                              // weights: constants, read ahead of the wait
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        gq[j] = a.d_q_gamma ? a.d_q_gamma[d + j] : 1.0f; gq[N + j] = a.d_q_gamma ? a.d_q_gamma[HALF + d + j] : 1.0f;
-        gk[j] = a.d_k_gamma ? a.d_k_gamma[d + j] : 1.0f; gk[N + j] = a.d_k_gamma ? a.d_k_gamma[HALF + d + j] : 1.0f;
-    }
+    for (int j = 0; j < 2 * N; ++j) gq[j] = gk[j] = 1.0f;
+    auto weights = [&](float *g, const float *from) {
+        if (!from) return;
+        *reinterpret_cast<float4 *>(g) = *reinterpret_cast<const float4 *>(from + d);
+        *reinterpret_cast<float4 *>(g + N) = *reinterpret_cast<const float4 *>(from + HALF + d);
+    };
+    weights(gq, a.d_q_gamma);
+    weights(gk, a.d_k_gamma);
     const float freq = a.d_inv_freq && threadIdx.x < HALF ? a.d_inv_freq[threadIdx.x] : 0.0f;
     pdl_wait();
     // all loads at once, the count's among them: rows up to max_rows exist, and what lies behind the last one is only not stored
     const int rows = *a.d_rows, slot = a.d_slot[m], pos = a.d_pos[m];
     const int heads = a.n_q + 2 * a.n_kv, h1 = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
-    const float *row = a.d_qkv + (long long)m * a.qkv_ld;
+    const float *row = a.d_qkv + (long long)m * a.qkv_ld + d;
     float x[STORE_AHEAD][2 * N];                             // heads on their way: the first ones under the angles
     auto load = [&](int h0) {
 #pragma unroll
         for (int k = 0; k < STORE_AHEAD; ++k) {
-            const int h = h0 + k * STORE_WARPS;
+            const int h = h0 + k * STEP;
             if (h < h1) {
-                *reinterpret_cast<F *>(x[k]) = *reinterpret_cast<const F *>(row + h * HD + d);
-                *reinterpret_cast<F *>(x[k] + N) = *reinterpret_cast<const F *>(row + h * HD + HALF + d);
+                *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(row + h * HD);
+                *reinterpret_cast<float4 *>(x[k] + N) = *reinterpret_cast<const float4 *>(row + h * HD + HALF);
             }
         }
     };
-    int h0 = blockIdx.y * heads_per_block + warp;
+    int h0 = blockIdx.y * heads_per_block + warp * HEADS + lane / LANES;
     load(h0);
     if (m >= rows) return;
     if (threadIdx.x < HALF && a.d_inv_freq) {
@@ -252,55 +251,61 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __g
     const bool in_pool = slot >= 0 && slot < a.n_pages * a.page;
     if (!in_pool && threadIdx.x == 0 && blockIdx.y == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
     __syncthreads();
+    float cs[N], sn[N];
+    *reinterpret_cast<float4 *>(cs) = *reinterpret_cast<const float4 *>(s_cos + d);
+    *reinterpret_cast<float4 *>(sn) = *reinterpret_cast<const float4 *>(s_sin + d);
     const int shift = 31 - __clz(a.page);
     const long long at = ((long long)(slot >> shift) * a.n_kv << shift) + (slot & (a.page - 1));       // of head 0: heads are a page apart
-    for (; h0 < h1; h0 += STORE_AHEAD * STORE_WARPS) {
+#pragma unroll 1
+    for (; __any_sync(0xffffffffu, h0 < h1); h0 += STORE_AHEAD * STEP) {
 #pragma unroll
         for (int k = 0; k < STORE_AHEAD; ++k) {
-            const int h = h0 + k * STORE_WARPS;
-            if (h >= h1) break;
-            if (h < a.n_q + a.n_kv) {
-                const bool is_q = h < a.n_q;
-                if (is_q ? a.d_q_gamma != nullptr : a.d_k_gamma != nullptr) {
-                    float ss = 0.0f;
+            const int h = h0 + k * STEP;
+            const bool is_q = h < a.n_q, turns = h < a.n_q + a.n_kv;
+            float ss = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 2 * N; ++j) ss = fmaf(x[k][j], x[k][j], ss);
-                    const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.eps);
+            for (int j = 0; j < 2 * N; ++j) ss = fmaf(x[k][j], x[k][j], ss);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (h >= h1) continue;
+            if (turns) {
+                if (is_q ? a.d_q_gamma != nullptr : a.d_k_gamma != nullptr) {
+                    const float inv = rsqrtf(fmaf(ss, 1.0f / (float)HD, a.eps));       // 2 ulp
 #pragma unroll
                     for (int j = 0; j < 2 * N; ++j) x[k][j] *= (is_q ? gq[j] : gk[j]) * inv;
                 }
                 if (a.d_inv_freq) {
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        const float cs = s_cos[d + j], sn = s_sin[d + j], lo = x[k][j], hi = x[k][N + j];
-                        x[k][j] = lo * cs - hi * sn; x[k][N + j] = lo * sn + hi * cs;
+                        const float lo = x[k][j], hi = x[k][N + j];
+                        x[k][j] = lo * cs[j] - hi * sn[j]; x[k][N + j] = lo * sn[j] + hi * cs[j];
                     }
                 }
             }
-            uint16_t b[2 * N];
-#pragma unroll
-            for (int j = 0; j < 2 * N; ++j) b[j] = to_bits<T>(x[k][j]);
             uint16_t *to;
-            if (h < a.n_q) to = static_cast<uint16_t *>(a.d_q) + (long long)m * a.q_ld + h * HD;
+            if (is_q) to = static_cast<uint16_t *>(a.d_q) + (long long)m * a.q_ld + h * HD;
             else {
-                const bool is_k = h < a.n_q + a.n_kv;
                 if (!in_pool) continue;
-                to = static_cast<uint16_t *>(is_k ? a.d_k_pool : a.d_v_pool) + (at + ((long long)(h - a.n_q - (is_k ? 0 : a.n_kv)) << shift)) * HD;
+                to = static_cast<uint16_t *>(turns ? a.d_k_pool : a.d_v_pool) + (at + ((long long)(h - a.n_q - (turns ? 0 : a.n_kv)) << shift)) * HD;
             }
-            H w[2];
-            memcpy(w, b, sizeof(w));
-            *reinterpret_cast<H *>(to + d) = w[0];
-            *reinterpret_cast<H *>(to + HALF + d) = w[1];
+            uint2 w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                w[j].x = (uint32_t)to_bits<T>(x[k][N * j]) | (uint32_t)to_bits<T>(x[k][N * j + 1]) << 16;
+                w[j].y = (uint32_t)to_bits<T>(x[k][N * j + 2]) | (uint32_t)to_bits<T>(x[k][N * j + 3]) << 16;
+            }
+            *reinterpret_cast<uint2 *>(to + d) = w[0];
+            *reinterpret_cast<uint2 *>(to + HALF + d) = w[1];
         }
-        if (h0 + STORE_AHEAD * STORE_WARPS < h1) load(h0 + STORE_AHEAD * STORE_WARPS);
+        load(h0 + STORE_AHEAD * STEP);
     }
 }
 
 template <typename T>
 int launch_store(const b200_paged_store_args &a, cudaStream_t st)
 {
-    // few rows: a warp to each head, or 32 rows would run on 32 SMs; many: all heads of a row in one block, which forms the angles once
-    const int heads = a.n_q + 2 * a.n_kv, per = a.max_rows <= 512 ? STORE_WARPS : heads;
+    // few rows: one round of heads to a block, or 32 rows would run on 32 SMs; many: all heads of a row in one block, which forms the angles once
+    const int heads = a.n_q + 2 * a.n_kv, per = a.max_rows <= 512 ? STORE_WARPS * 256 / a.hd : heads;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.max_rows, (heads + per - 1) / per);
     cfg.blockDim = dim3(STORE_WARPS * 32);
