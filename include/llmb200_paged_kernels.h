@@ -19,11 +19,13 @@
  *              page of a request is not read
  *   slot       number of a token's place in a pool: page number * page + place within the page
  *   rows       the new tokens of all requests, request after request: request r has rows d_row_start[r] ..
- *              d_row_start[r + 1] - 1. Rows behind the last request's are neither read nor written.
+ *              d_row_start[r + 1] - 1. Rows behind the last request's, up to max_rows, exist in every array of rows, are
+ *              never written, and what they hold has no influence.
  *
  * Every function enqueues on `stream` (a cudaStream_t) of the current device and returns 0, a positive cudaError_t, or a
  * negative B200_E_* code for rejected arguments; nothing allocates or waits. What only the device can see is reported
- * through *d_status (optional): bits are added to it, never taken away.
+ * through *d_status (optional): bits are added to it, never taken away. Arrays that are written overlap no other array
+ * of the call, but where it is said.
  */
 #ifndef LLMB200_PAGED_KERNELS_H
 #define LLMB200_PAGED_KERNELS_H
@@ -113,7 +115,7 @@ int b200_paged_store(const b200_paged_store_args *a, void *stream);
  * ---------------------------------------------------------------------- */
 typedef struct b200_paged_attn_args {
     int wtype, n_q, n_kv, hd, page, n_pages, max_rows;
-    float scale;
+    float scale;                                             /* finite */
     const void *d_q; long long q_ld;                         /* rows q_ld elements apart, a multiple of 8; 16-byte aligned */
     const void *d_k_pool, *d_v_pool;
     void *d_out; long long out_ld;                           /* likewise; n_q * hd elements of the pool's type a row */

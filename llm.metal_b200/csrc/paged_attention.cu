@@ -5,14 +5,19 @@
 #include "paged_attention_many.cuh"
 
 #include <atomic>
+#include <cmath>
 
 extern unsigned long long g_b200_launches;
 
 namespace {
 
 constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 4;
-// Sets of more query rows than FEW_MOST go the second way, where hd is one of its own; a request of BIG_ROWS of them fills a stream there by itself.
-constexpr int FEW_MOST = 16, BIG_ROWS = 128;
+// Sets of more query rows than FEW_MOST go the second way, where hd is one of its own (two tiles of 16 rows read their keys twice, mostly from L2). Us, hd 128,
+// 8 key / value heads, by single warps and on tcgen05: 8 requests of 6000 tokens, 32 query rows each 54 and 66, 48 rows 74 and 70, 64 rows 134 and 70; 64 of
+// 1500 tokens, 32 rows 137 and 132, 48 rows 217 and 140; hd 64, 64 requests of 32 rows 74 and 107, of 48 rows 124 and 115.
+// A request of BIG_ROWS query rows fills a stream there by itself: portions that met prefix and own tokens in two sets, and were joined, took 520 us
+// where one set takes 287 (four requests of 125 .. 811 new tokens behind 4096).
+constexpr int FEW_MOST = 32, BIG_ROWS = 128;
 
 __host__ __device__ constexpr int block_threads(int hd) { return hd > 128 ? 128 : MANY_THREADS; }
 __host__ __device__ constexpr int few_warps(int hd) { return hd > 128 ? 4 : 8; }
@@ -183,7 +188,7 @@ Layout layout_of(const b200_paged_attn_args &a)
     Layout L = {};
     L.shape.by_g = div_of((int)G); L.shape.by_kv = div_of(a.n_kv);
     L.shape.few_most = wide ? FEW_MOST : INT_MAX; L.shape.big = wide ? BIG_ROWS : INT_MAX;
-    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;
+    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;              // from the ends of both kinds of blocks, 64 requests of one prefix of 65521 tokens: together within a tenth
     L.shape.row_step[0] = (int)((FEW_ROWS * 256 + G - 1) / G); L.shape.row_step[1] = (int)((MANY_ROWS * 256 + G - 1) / G);
     L.shape.each = 1;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
@@ -259,6 +264,7 @@ extern "C" int b200_paged_attn(const b200_paged_attn_args *ap, void *stream)
     if (!ap) return B200_E_BADARG;
     const b200_paged_attn_args &a = *ap;
     if (const int rc = check_sizes(a)) return rc;
+    if (!std::isfinite(a.scale)) return B200_E_BADARG;
     if (a.max_rows == 0 || a.n_req == 0) return 0;
     if (!a.d_q || !a.d_k_pool || !a.d_v_pool || !a.d_out || !a.d_row_start || !a.d_len || !a.d_table || !a.d_work) return B200_E_BADARG;
     if (a.n_groups && (!a.d_group_start || !a.d_prefix_len || (a.prefix_ld && !a.d_prefix_table))) return B200_E_BADARG;

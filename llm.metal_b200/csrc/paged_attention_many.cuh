@@ -204,7 +204,8 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
         // ---- a stream's rows ----
         const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;       // stream, row of its tile = lane of tensor memory
         const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), o_at = tm + O_COL + s * 128;
-        const float c = fabsf(a.scale) * 1.4426950408889634f;            // the sign goes into the queries
+        // the sign goes into the queries; a scale of zero weighs all seen keys alike, and hidden ones, at minus infinity, not at all
+        const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.17549435e-38f);
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         uint32_t turn = 0, item = 0, s_phase = 0, even = 0, odd = 0, alone_phase = 0, both_phase = 0;      // even, odd: products with weights of the first and of the second place, before this piece
         bool ok = true;

@@ -216,19 +216,21 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
         int n = 0, k = 0;
         const int way = way_of(plan, s);
         if (s.nr > 0 && s.keys > 0) {
-            float cost;
+            float cost, most;                                // most: of a head, in floating point: lines of 2^31 units are refused below
             if (way) {
                 k = tiles_of<1>(s);
                 n = line_before<1>(plan, s, k);
                 // a tile whose rows fit into one stream costs two thirds
                 const int last = s.nr - (k - 1) * Cut<1>::ROWS;
+                most = (float)k * (float)(Cut<1>::GAP + 1 + units_of<1>(plan, s, k - 1));
                 cost = (float)n * shape.ratio * (last > Cut<1>::ROWS / 2 ? 1.0f : 1.0f - __fdividef(0.35f, (float)k));
             } else {
                 k = tiles_of<0>(s);
                 n = line_before<0>(plan, s, k);
                 cost = (float)n;
+                most = (float)k * (float)(Cut<0>::GAP + 1 + units_of<0>(plan, s, k - 1));
             }
-            size += (float)n * (float)shape.by_kv.d;
+            size += most * (float)shape.by_kv.d;
             if (way) many_cost += cost * (float)shape.by_kv.d;
             n *= shape.by_kv.d; k *= shape.by_kv.d;
         }

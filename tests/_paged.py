@@ -24,9 +24,10 @@ class Step:
     """Pools, tables, rows and the argument structure of an attention call. `fill`: what unseen slots hold."""
 
     def __init__(self, pkg, dtype, n_q, n_kv, hd, page, total, new, groups=(), prefix=(), seed=0, fill=float("nan"), spare=3, q_scale=2.0,
-                 first_page=0, q_pad=0, out_pad=0, table_pad=1, max_rows=None):
+                 first_page=0, q_pad=0, out_pad=0, table_pad=1, max_rows=None, scale=None):
         self.pkg, self.lib = pkg, pkg.lib()
         self.n_q, self.n_kv, self.hd, self.page, self.total, self.new = n_q, n_kv, hd, page, list(total), list(new)
+        self.scale = hd ** -0.5 if scale is None else scale
         self.groups, self.prefix = list(groups), list(prefix)       # first request of every group and the end; prefixes
         self.type, wtype = TYPES[dtype]
         g = torch.Generator(device="cuda").manual_seed(seed)
@@ -61,7 +62,7 @@ class Step:
         self.q[:self.rows, :n_q * hd] = (q_scale * torch.randn(self.rows, n_q * hd, generator=g, device="cuda")).to(self.type)
         self.out = torch.full((self.max_rows, n_q * hd + out_pad), 7.0, dtype=self.type, device="cuda")
         self.status = ints([0])
-        self.a = args(pkg.PagedAttnArgs, wtype=wtype, n_q=n_q, n_kv=n_kv, hd=hd, page=page, n_pages=n_pages, max_rows=self.max_rows, scale=hd ** -0.5,
+        self.a = args(pkg.PagedAttnArgs, wtype=wtype, n_q=n_q, n_kv=n_kv, hd=hd, page=page, n_pages=n_pages, max_rows=self.max_rows, scale=self.scale,
                       d_q=self.q, q_ld=self.q.shape[1], d_k_pool=self.k, d_v_pool=self.v, d_out=self.out, out_ld=self.out.shape[1],
                       n_req=len(self.new), d_row_start=ints(self.ends), d_len=ints(self.total), d_table=self.table, table_ld=ld,
                       n_groups=len(self.prefix), d_group_start=ints(self.groups or [0]), d_prefix_len=ints(self.prefix or [0]), d_prefix_table=self.p_table, prefix_ld=p_ld,
@@ -109,8 +110,8 @@ class Step:
             kept_k, kept_v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
             for h in range(self.n_q):
                 i = h // (self.n_q // self.n_kv)
-                z = (q[:, h] @ k[i].T * self.hd ** -0.5).masked_fill(hidden, -math.inf)
-                size = (q[:, h].abs() @ kept_k[i].abs().T * self.hd ** -0.5).masked_fill(hidden, 0)
+                z = (q[:, h] @ k[i].T * self.scale).masked_fill(hidden, -math.inf)
+                size = (q[:, h].abs() @ kept_k[i].abs().T * abs(self.scale)).masked_fill(hidden, 0)
                 w = torch.softmax(z, -1)
                 terms = torch.where(hidden[..., None], 0.0, w[..., None] * v[i]) if not torch.isfinite(v[i]).all() else None
                 want = terms.sum(1) if terms is not None else w @ v[i]

@@ -74,7 +74,8 @@ def test_store_refusals(pkg, lib, more, code):
     (dict(d_out=None), BADARG), (dict(d_row_start=None), BADARG), (dict(d_len=None), BADARG), (dict(d_table=None), BADARG), (dict(d_group_start=None), BADARG),
     (dict(d_prefix_len=None), BADARG), (dict(d_prefix_table=None), BADARG), (dict(d_work=None), BADARG), (dict(d_work=P + 8), BADARG), (dict(d_out=P + 8), BADARG),
     (dict(out_ld=500), BADARG), (dict(out_ld=518), BADARG), (dict(n_req=-1), BADARG), (dict(n_req=1025), BADARG), (dict(n_groups=-1), BADARG), (dict(n_groups=5), BADARG),
-    (dict(table_ld=-1), BADARG), (dict(table_ld=(1 << 20) + 1), BADARG), (dict(prefix_ld=(1 << 20) + 1), BADARG), (dict(work_bytes=100), BADARG)])
+    (dict(table_ld=-1), BADARG), (dict(table_ld=(1 << 20) + 1), BADARG), (dict(prefix_ld=(1 << 20) + 1), BADARG), (dict(work_bytes=100), BADARG),
+    (dict(scale=float("nan")), BADARG), (dict(scale=-float("inf")), BADARG)])
 def test_attention_refusals(pkg, lib, more, code):
     assert lib.b200_paged_attn(C.byref(attn(pkg, **more)), None) == code
     assert lib.b200_paged_attn(None, None) == BADARG

@@ -307,6 +307,23 @@ def test_scores_of_all_sizes(pkg):
         s.check()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.7])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_scales(pkg, scale, hd):
+    s = Step(pkg, "bf16", 8, 2, hd, 128, [500, 260, 3], [1, 130, 3], [0, 3], [300], scale=scale)
+    s.run()
+    s.check()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_of_all_sizes_hold_shared_prefixes(pkg, page, hd):
+    for prefix in (1, 63, 64, 65, 257, 1000):
+        s = Step(pkg, "f16", 16, 2, hd, page, [page, 1, page + 1, 2 * page - 1] * 3, [1] * 12, [0, 12], [prefix], seed=prefix)
+        s.run()
+        s.check()
+
+
 @pytest.mark.parametrize("q_pad,out_pad", [(8, 16), (136, 0)])
 def test_attention_strides(pkg, q_pad, out_pad):
     s = Step(pkg, "bf16", 16, 8, 128, 16, [50, 300, 9], [1, 5, 9], [0, 3], [70], q_pad=q_pad, out_pad=out_pad, table_pad=5)
@@ -334,6 +351,36 @@ def test_same_bits_again_and_on_another_stream(pkg):
         s.run(side.cuda_stream)
         side.synchronize()
         assert torch.equal(s.out, want)
+
+
+def test_the_first_call_may_be_a_captured_one(pkg):
+    """In a process of its own: nothing was launched before the capture."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys; sys.path[:0] = [%r, %r]\nimport torch, __graft_entry__ as e\nfrom _paged import Step\n"
+            "s = Step(e.load_package(), 'f16', 8, 2, 128, 16, [40, 700], [1, 90], [0, 2], [100])\ntorch.cuda.synchronize()\ng = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g): s.run(torch.cuda.current_stream().cuda_stream)\n"
+            "assert (s.out == 7).all()\nfor _ in range(3): g.replay()\ntorch.cuda.synchronize()\ns.check()\nprint('fine')\n") % (here, os.path.dirname(here))
+    r = subprocess.run([sys.executable, "-c", code], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-2000:]
+
+
+def test_two_calls_at_once(pkg):
+    """On two streams, each with its own d_work: as alone."""
+    steps = [Step(pkg, "bf16", 32, 8, 128, 16, [900, 1, 260] * 5, [1, 1, 60] * 5, [0, 15], [3000], seed=k) for k in (1, 2)]
+    want = [s.run().clone() for s in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    for s in steps:
+        s.out.fill_(7.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, at in zip(steps, streams):
+            s.run(at.cuda_stream)
+    torch.cuda.synchronize()
+    for s, w in zip(steps, want):
+        assert torch.equal(s.out, w) and s.status.tolist() == [0]
 
 
 @pytest.mark.parametrize("field,values", [
