@@ -20,9 +20,11 @@ constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 4;
 constexpr int FEW_MOST = 32, BIG_ROWS = 128;
 
 __host__ __device__ constexpr int block_threads(int hd) { return hd > 128 ? 128 : MANY_THREADS; }
-__host__ __device__ constexpr int few_warps(int hd) { return hd > 128 ? 4 : 8; }
+__host__ __device__ constexpr int most_few_warps(int hd) { return hd > 128 ? 4 : 8; }
 
 struct Room { int slots, plan_off; };
+// Dynamic shared memory: what is left of an SM's besides static memory and the alignment to 1024 bytes.
+constexpr size_t ROOM = 227 * 1024 - 2048 - 1024;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(block_threads(HD), 1)
@@ -36,11 +38,14 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     pdl_wait();
     pdl_launch_dependents();                                 // after the wait: attn_join_kernel reads the lengths ahead of its own
     if (!make_plan(a, shape, base + room.plan_off, plan)) return;
-    if constexpr (HD > 128) few_worker<T, HD>(a, plan, few, blockIdx.x * few_warps(HD) + warp, smem_u32(base) + warp * few_ring(HD));
+    if constexpr (HD > 128) {
+        if (warp < shape.few_warps) few_worker<T, HD>(a, plan, few, blockIdx.x * shape.few_warps + warp, smem_u32(base) + warp * few_ring(HD));
+    }
     else if ((int)blockIdx.x < plan.many_blocks) many_block<T, HD>(map_k, map_v, a, plan, many, base, room.slots);
     else if (warp >= 4) {                                    // registers as in many_block
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        few_worker<T, HD>(a, plan, few, ((int)blockIdx.x - plan.many_blocks) * few_warps(HD) + warp - 4, smem_u32(base) + (warp - 4) * few_ring(HD));
+        if (warp - 4 < shape.few_warps)
+            few_worker<T, HD>(a, plan, few, ((int)blockIdx.x - plan.many_blocks) * shape.few_warps + warp - 4, smem_u32(base) + (warp - 4) * few_ring(HD));
     } else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
 }
 
@@ -188,12 +193,15 @@ Layout layout_of(const b200_paged_attn_args &a)
     Layout L = {};
     L.shape.by_g = div_of((int)G); L.shape.by_kv = div_of(a.n_kv);
     L.shape.few_most = wide ? FEW_MOST : INT_MAX; L.shape.big = wide ? BIG_ROWS : INT_MAX;
-    L.shape.blocks = sm_count(); L.shape.few_warps = few_warps(a.hd); L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;              // from the ends of both kinds of blocks, 64 requests of one prefix of 65521 tokens: together within a tenth
+    L.shape.blocks = sm_count(); 
+    const int rings = (int)((ROOM - plan_bytes(a.n_req, a.n_groups)) / few_ring(a.hd));       // hundreds of requests leave less than all of the warps a ring
+    L.shape.few_warps = rings < most_few_warps(a.hd) ? rings : most_few_warps(a.hd);
+    L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;              // from the ends of both kinds of blocks, 64 requests of one prefix of 65521 tokens: together within a tenth
     L.shape.row_step[0] = (int)((FEW_ROWS * 256 + G - 1) / G); L.shape.row_step[1] = (int)((MANY_ROWS * 256 + G - 1) / G);
     L.shape.each = 1;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker
     const long long few_tiles = sets * ((FEW_MOST + FEW_ROWS - 1) / FEW_ROWS), full = (all + FEW_ROWS - 1) / FEW_ROWS + sets;
-    const long long few_slots = (wide && few_tiles < full ? few_tiles : full) * a.n_kv + L.shape.blocks * L.shape.few_warps;
+    const long long few_slots = (wide && few_tiles < full ? few_tiles : full) * a.n_kv + L.shape.blocks * most_few_warps(a.hd);
     const long long many_sets = all / (FEW_MOST + 1) < sets ? all / (FEW_MOST + 1) : sets;
     const long long many_slots = wide && all > FEW_MOST ? ((all + MANY_ROWS - 1) / MANY_ROWS + many_sets) * a.n_kv + L.shape.blocks : 0;
     L.few_acc = 0;
@@ -212,19 +220,18 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     char *work = static_cast<char *>(a.d_work);
     const Pieces few = {reinterpret_cast<float *>(work + L.few_acc), reinterpret_cast<float2 *>(work + L.few_top)};
     const Pieces many = {reinterpret_cast<float *>(work + L.many_acc), reinterpret_cast<float2 *>(work + L.many_top)};
-    const size_t plan = plan_bytes(a.n_req, a.n_groups), rings = (size_t)few_warps(HD) * few_ring(HD);
+    const size_t plan = plan_bytes(a.n_req, a.n_groups), rings = (size_t)L.shape.few_warps * few_ring(HD);
     Room room = {0, (int)rings};
     CUtensorMap map_k = {}, map_v = {};
     if constexpr (HD <= 128) {
         constexpr size_t SLOT = KEY64 * (HD / 64), QUERIES = 2 * QUERY64 * (HD / 64);
-        const size_t left = 227 * 1024 - 1024 - 2048 - plan - QUERIES;      // but for the alignment, the static memory, the plan and the queries
+        const size_t left = ROOM - plan - QUERIES;
         room.slots = (int)(left / SLOT) < MOST_SLOTS ? (int)(left / SLOT) : MOST_SLOTS;
         if (QUERIES + room.slots * SLOT > rings) room.plan_off = (int)(QUERIES + room.slots * SLOT);
         const int box = a.page < MANY_KEYS ? a.page : MANY_KEYS;
         if (!pool_map(&map_k, a.d_k_pool, a, box) || !pool_map(&map_v, a.d_v_pool, a, box)) return B200_E_STATE;
     }
     const size_t smem = room.plan_off + plan + 1024;
-    if (smem > 227 * 1024 - 2048) return B200_E_TOOLARGE;
     static std::atomic<unsigned long long> pages_done, join_done;
     cudaError_t e = allow_all(attn_pages_kernel<T, HD>, pages_done);
     if (e == cudaSuccess) e = allow_all(attn_join_kernel<T, HD>, join_done);

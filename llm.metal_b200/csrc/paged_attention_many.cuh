@@ -137,15 +137,18 @@ template <typename T, int HD> __device__ __noinline__ void add_key(uint32_t s_at
 // Which units of a piece a stream has, and the order in which the piece's keys and values pass through the ring: `lead` units of keys, then values and keys by turns.
 struct Streams {
     bool halves;                         // one tile of rows, every other unit to a stream
-    int units[2], n, lead;
+    int units[2], n, lead, ahead;        // lead: `ahead`, or all that there are
     __device__ __forceinline__ uint32_t values(int j) const { return lead + j + min(j, n - lead); }
 };
-__device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q)
+// (Four units ahead where every other one is a stream's, if the ring has 7 places: the values of a unit whose scores are there then lie in a place whose
+// occupant before them has arrived, so that the parity of its barrier says which of the two is meant.)
+__device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q, int slots)
 {
     Streams w;
     w.n = q.n;
     w.halves = min(MANY_ROWS, q.s.nr - q.t * MANY_ROWS) <= HALF_ROWS;
-    w.lead = min(q.n, w.halves ? 4 : 2);
+    w.ahead = w.halves && slots >= 7 ? 4 : 2;
+    w.lead = min(q.n, w.ahead);
     if (w.halves) { w.units[0] = (q.n + 1) / 2; w.units[1] = q.n / 2; return w; }
     const int seen = q.s.own ? q.s.keys - q.s.rows + over(q.t * MANY_ROWS + HALF_ROWS - 1, p.shape.by_g) + 1 : q.s.keys;
     w.units[0] = max(0, min(q.n, units_before_own<1>(q.s) + (seen + MANY_KEYS - 1) / MANY_KEYS - q.k0));
@@ -212,7 +215,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
         Walk<1> walk(p, blockIdx.x);
         Piece piece;
         while (ok && walk.next(p, piece)) {
-            const Streams w = streams_of(p, piece);
+            const Streams w = streams_of(p, piece, slots);
             const Set &st = piece.s;
             const int i0 = piece.t * MANY_ROWS, i = i0 + (w.halves ? 0 : s * HALF_ROWS) + r, mine = w.units[s];
             const bool valid = i < st.nr, warp_valid = __any_sync(0xffffffffu, valid);
@@ -419,7 +422,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             Walk<1> walk(p, blockIdx.x);
             Piece piece;
             while (ok && walk.next(p, piece)) {
-                const Streams w = streams_of(p, piece);
+                const Streams w = streams_of(p, piece, slots);
                 const int n = piece.n, lead = w.lead;
                 const Keys keys = keys_of<1>(a, p, piece);
                 struct Unit { int there, y, id; };               // copies, the first token in the page, this lane's page
@@ -468,8 +471,8 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             const uint32_t s_at = tmem + S_COL + s * 128, o_at = tmem + O_COL + s * 128;
             auto arrived = [&](uint64_t *bar, uint32_t phase) { return (bool)__all_sync(0xffffffffu, wait_or_abort(bar, phase, abort_flag)); };
             while (ok && walk.next(p, piece)) {
-                const Streams w = streams_of(p, piece);
-                const int n = uniform(piece.n), mine = uniform(w.units[s]), lead = uniform(w.lead), halves = uniform(w.halves);
+                const Streams w = streams_of(p, piece, slots);
+                const int n = uniform(piece.n), mine = uniform(w.units[s]), lead = uniform(w.lead), ahead = uniform(w.ahead), halves = uniform(w.halves);
                 const uint64_t q_desc = smem_desc_sw128(q_tiles + (halves ? 0 : s * Q_TILE));
                 ok = arrived(&q_bar[0], turn & 1) && arrived(&q_bar[1], turn & 1);
                 ++turn;
@@ -518,8 +521,8 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     for (int u = 0; u < n && ok; ++u) {
                         if ((u & 1) == s) sums((u >> 1) & 1, at);
                         at.next(slots);
-                        if (u + 4 < n) {
-                            if ((u & 1) == s) scores((u >> 1) & 1, at);
+                        if (u + ahead < n) {
+                            if ((u & 1) == s) scores(((u + ahead) >> 1) & 1, at);
                             at.next(slots);
                         }
                     }

@@ -47,7 +47,7 @@ namespace {
 // The two ways: rows of a tile, keys of a unit, fewest units of a worker, units' worth of a gap (two at least: see line_before).
 template <int WAY> struct Cut;
 template <> struct Cut<0> { static constexpr int ROWS = 16, KEYS = 16, LEAST = 4, GAP = 2; };
-template <> struct Cut<1> { static constexpr int ROWS = 256, KEYS = 64, LEAST = 4, GAP = 6; };
+template <> struct Cut<1> { static constexpr int ROWS = 256, KEYS = 64, LEAST = 8, GAP = 8; };
 
 // What a block knows of the step, in shared memory.
 struct Plan {

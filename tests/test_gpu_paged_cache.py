@@ -277,6 +277,17 @@ def test_attention_of_the_most_requests(pkg, dtype):
     s.check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_of_the_most_groups(pkg, hd):
+    """As many groups as requests: the largest plan, which leaves the fewest places for keys and values."""
+    rng = random.Random(6)
+    new = [rng.choice([0, 1, 1, 1, 9, 20]) if r % 50 else 70 for r in range(1024)]
+    total = [a + rng.randint(0, 90) for a in new]
+    s = Step(pkg, "f16", 4, 1, hd, 16, total, new, list(range(1025)), [rng.choice([0, 3, 200, 333]) for _ in range(1024)], seed=10)
+    s.run()
+    s.check()
+
+
 @pytest.mark.parametrize("fill", [float("inf"), -float("inf"), 0.0])
 def test_attention_with_other_unseen_slots(pkg, fill):
     s = Step(pkg, "f16", 8, 2, 128, 32, [33, 70, 5], [1, 40, 5], [0, 2], [100], fill=fill)
