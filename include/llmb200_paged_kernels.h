@@ -83,6 +83,7 @@ int b200_pages_release(const b200_pages_args *a, void *stream);
  *          (d, d + hd / 2) turns by the angle d_pos[m] * d_inv_freq[d], formed exactly (d_inv_freq NULL: no rotation)
  *   k, v   rounded to the pool's type, stored at slot d_slot[m]; a slot outside the pool is left out
  *   q      rounded likewise, stored to row m of d_q: what b200_paged_attn reads
+ * With use_pdl the weights (d_q_gamma, d_k_gamma, d_inv_freq) are read ahead of the wait for the kernel before.
  * *d_rows rows (a device word, at most max_rows): the last of b200_pages_extend's d_row_start. Two rows of one slot: one
  * of them is kept.
  * ---------------------------------------------------------------------- */
@@ -105,7 +106,8 @@ int b200_paged_store(const b200_paged_store_args *a, void *stream);
  *   out[m][h] = sum over those keys of softmax(scale * q[m][h] . k) v,   head h reads key / value head h / (n_q / n_kv)
  * Group g is the requests d_group_start[g] .. d_group_start[g + 1] - 1, its prefix the first d_prefix_len[g] tokens (0:
  * none) of the pages d_prefix_table[g][prefix_ld]. Requests outside every group have no prefix; n_groups 0: no
- * request has. The pages of a prefix are read once for all rows of its group, as far as they fit into tiles.
+ * request has. The pages of a prefix are read once for every 256 query rows (rows times n_q / n_kv) of its group, up to hd 128, and
+ * for every 16 above; a request that brings 128 of them by itself, a portion of a prompt, reads its prefix for itself.
  * Tokens that a row does not see have no influence on it, whatever their slots hold (infinities and NaN too).
  *
  * If a length or a range does not fit its buffer, the call leaves all of its output as it was and *d_status says

@@ -3,7 +3,8 @@
 // Tables (extend, release): prefix sums over at most 1024 requests, one a thread, and then one (row or page) a thread, which finds its request by
 // bisection in shared memory. A step of 32 requests is two dependent round trips to L2 and a launch; large ones are stores. One cluster of blocks:
 // all of them scan for themselves, and nothing that was read is written before all have read it, so that lengths and the stack's height
-// can be updated in place. Whole numbers throughout: the same result in every run.
+// can be updated in place. Whole numbers throughout: the same result in every run. A step of 32 requests is bound by its launch (7 us with the host's part), 1000
+// requests with 100 000 new tokens take 14 us (20 with an entry at a time to a thread), 90 000 pages given back 10.
 #include "stream_core.cuh"
 #include "../../include/llmb200_paged_kernels.h"
 
@@ -105,14 +106,16 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
         }
     }
     if (why) return;
-    // Four at a time: one search, one round trip to the table and the stack, and 16-byte stores where the arrays are aligned for them.
-    const int first = 4 * (blockIdx.x * blockDim.x + threadIdx.x), step = 4 * gridDim.x * blockDim.x, shift = 31 - __clz(a.page);
+    // Where there is more than one to a thread, four at a time: one search, one round trip to the table and the stack, and 16-byte stores where the arrays are
+    // aligned for them.
+    const int thread = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x, shift = 31 - __clz(a.page);
+    const int pages_each = total.y > threads ? 4 : 1, rows_each = total.x > threads ? 4 : 1;
 #pragma unroll 1
-    for (int p = first; p < total.y; p += step) {
+    for (int p = pages_each * thread; p < total.y; p += pages_each * threads) {
         int q = owner_of(s_page, n, p);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (p + k >= total.y) break;
+            if (k >= pages_each || p + k >= total.y) break;
             while (q + 1 < n && s_page[q + 1] <= p + k) ++q;
             if (RELEASE) a.d_free[free_n + p + k] = a.d_table[(size_t)q * a.table_ld + (p + k - s_page[q])];
             else a.d_table[(size_t)q * a.table_ld + ((s_len[q] + a.page - 1) >> shift) + (p + k - s_page[q])] = a.d_free[free_n - 1 - p - k];
@@ -122,10 +125,11 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
     unsigned outside = 0;
     const bool wide = ((reinterpret_cast<uintptr_t>(a.d_slot) | reinterpret_cast<uintptr_t>(a.d_pos)) & 15) == 0;
 #pragma unroll 1
-    for (int m = first; m < total.x; m += step) {
+    for (int m = rows_each * thread; m < total.x; m += rows_each * threads) {
         int q = owner_of(s_row, n, m), slot[4], pos[4], token_in_page[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            if (k >= rows_each) break;
             const int at_row = min(m + k, total.x - 1);
             while (q + 1 < n && s_row[q + 1] <= at_row) ++q;
             const int token = s_len[q] + (at_row - s_row[q]), page = token >> shift, held = (s_len[q] + a.page - 1) >> shift;
@@ -136,17 +140,18 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            if (k >= rows_each) break;
             const bool ok = slot[k] >= 0 && slot[k] < a.n_pages;
             slot[k] = ok ? (slot[k] << shift) + token_in_page[k] : -1;
             if (!ok) outside = B200_PAGED_BAD_PAGE;
         }
-        if (wide && m + 4 <= total.x) {
+        if (rows_each == 4 && wide && m + 4 <= total.x) {
             *reinterpret_cast<int4 *>(a.d_slot + m) = make_int4(slot[0], slot[1], slot[2], slot[3]);
             *reinterpret_cast<int4 *>(a.d_pos + m) = make_int4(pos[0], pos[1], pos[2], pos[3]);
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (m + k < total.x) { a.d_slot[m + k] = slot[k]; a.d_pos[m + k] = pos[k]; }
+                if (k < rows_each && m + k < total.x) { a.d_slot[m + k] = slot[k]; a.d_pos[m + k] = pos[k]; }
         }
     }
     report(a.d_status, outside);
@@ -190,11 +195,10 @@ int launch_pages(const b200_pages_args *ap, void *stream)
 }
 
 // ---- new rows into their slots ------------------------------------------------------------------------------------------------
-// Bound by memory: 4 bytes read and 2 written a number. hd / 8 lanes hold a head, each four numbers of its lower half and the four that they turn with, so that
-// the norm is a shuffle or two and the rotation stays in the lane. (A warp to a head of 128, four numbers a lane, took 140 instructions a head, and
-// 8191 rows of 32 heads 50 us.) The angle pos * inv_freq is formed in 64 bits (exact) and brought into one turn before the
-// 32-bit sine and cosine: as a 32-bit product it is off by pos * 2^-24, more than binary16's step from position 8000 on. One a lane pair and
-// block. q, k and v are rounded once, to the type of the cache that the tensor cores read.
+// Bound by memory: 4 bytes read and 2 written a number; 8191 rows of 32 heads of 128 take 46 us, 4.4 TB/s, where a copy reaches 6.6. hd / 8 lanes hold a
+// head, each four numbers of its lower half and the four that they turn with, so that the norm is a few shuffles and the rotation stays in
+// the lane. (A warp to a head of 128, four numbers a lane: 140 instructions a head, 50 us.) The angle pos * inv_freq is formed in 64 bits (exact) and brought
+// into one turn before the 32-bit sine and cosine: as a 32-bit product it is off by pos * 2^-24, more than binary16's step from position 8000 on. q, k and v are rounded once, to the type of the cache that the tensor cores read.
 template <typename T> __device__ __forceinline__ uint16_t to_bits(float x)
 {
     if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rn(x));
