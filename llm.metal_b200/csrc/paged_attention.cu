@@ -12,7 +12,7 @@ extern unsigned long long g_b200_launches;
 
 namespace {
 
-constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 4;
+constexpr int JOIN_WARPS = 4, JOIN_BLOCKS = 4, JOIN_CHUNK = 8;
 // Sets of more query rows than FEW_MOST go the second way, where hd is one of its own (two tiles of 16 rows read their keys twice, mostly from L2). Us, hd 128,
 // 8 key / value heads, by single warps and on tcgen05: 8 requests of 6000 tokens, 32 query rows each 54 and 66, 48 rows 74 and 70, 64 rows 134 and 70; 64 of
 // 1500 tokens, 32 rows 137 and 132, 48 rows 217 and 140; hd 64, 64 requests of 32 rows 74 and 107, of 48 rows 124 and 115.
@@ -69,7 +69,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_constant__ Shape shape, const Pieces few, const Pieces many)
 {
-    constexpr int N = HD / 32, AHEAD = HD > 128 ? 4 : 8;     // numbers of a lane, next to one another; pieces on their way
+    constexpr int N = HD / 32, AHEAD = 8;                    // numbers of a lane, next to one another; pieces on their way
     extern __shared__ __align__(1024) char smem[];
     __shared__ Plan p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -77,69 +77,193 @@ attn_join_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_co
     if (!make_plan(a, shape, smem, p)) { pdl_wait(); return; }
     pdl_launch_dependents();
     bool waited = false;
-    const int G = shape.by_g.d, rows = p.row[p.n_req], workers = gridDim.x * JOIN_WARPS;
-    // an item is a row and a query head, or all of those of a key / value head where there are more than warps
-    const int heads = (long long)rows * a.n_q > workers ? G : 1, per_row = heads == 1 ? a.n_q : a.n_kv;
-    for (long long at = blockIdx.x * JOIN_WARPS + warp; at < (long long)rows * per_row; at += workers) {
-        const int row = (int)(at / per_row), first = (int)(at % per_row) * heads, h = over(first, shape.by_g), r = last_at(p.row, p.n_req, row);
+    const int G = shape.by_g.d, all = p.row[p.n_req] * a.n_q, workers = gridDim.x * JOIN_WARPS;
+#pragma unroll 1
+    for (int at = blockIdx.x * JOIN_WARPS + warp; at < all; at += workers) {
+        const int row = at / a.n_q, head = at - row * a.n_q, h = over(head, shape.by_g), r = last_at(p.row, p.n_req, row);
         int group = group_of(p, r);
         const Set own = set_at(p, p.n_groups + r);
         if (own.before > 0) group = -1;                      // one set
-        const Set shared = set_at(p, max(group, 0));
+        const int i = (row - p.row[r]) * G + head - h * G;
+        Cuts x = {}, y = way_of(p, own) ? cuts_of<1>(p, own, many, p.n_groups + r, h, i, HD) : cuts_of<0>(p, own, few, p.n_groups + r, h, i, HD);
+        if (group >= 0) {
+            const Set shared = set_at(p, group);
+            const int j = i + (p.small[r] - p.small[p.group[group]]) * G;
+            x = way_of(p, shared) ? cuts_of<1>(p, shared, many, group, h, j, HD) : cuts_of<0>(p, shared, few, group, h, j, HD);
+        }
+        x.acc += lane * N; y.acc += lane * N;
+        if (group < 0 && !y.several) continue;           // stored where it was formed
+        if (!waited) { pdl_wait(); waited = true; }
+        const int n = x.count + y.count;
+        auto top_of = [&](int j) { return j < x.count ? x.top + (long long)j * x.step : y.top + (long long)(j - x.count) * y.step; };
+        auto acc_of = [&](int j) { return j < x.count ? x.acc + (long long)j * x.step * HD : y.acc + (long long)(j - x.count) * y.step * HD; };
+        float top = -INFINITY, l = 0.0f, o[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] = 0.0f;
+#pragma unroll 1
+        for (int j0 = 0; j0 < n; j0 += AHEAD) {
+            float2 ml[AHEAD];
+            float v[AHEAD][N];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {            // behind the last one it again, with no weight
+                const int k = min(j0 + j, n - 1);
+                const float *from = acc_of(k);
+                ml[j] = *top_of(k);
+                if constexpr (N >= 4) {
+#pragma unroll
+                    for (int q = 0; q < N; q += 4) *reinterpret_cast<float4 *>(&v[j][q]) = *reinterpret_cast<const float4 *>(from + q);
+                } else *reinterpret_cast<float2 *>(v[j]) = *reinterpret_cast<const float2 *>(from);
+            }
+            asm volatile("" ::: "memory");                  // all of them before the first is used: left to itself the compiler puts each before its use
+            float higher = top;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) higher = fmaxf(higher, ml[j].x);
+            const float base = higher == -INFINITY ? 0.0f : higher, down = ex2(top - base);
+            top = higher;
+            l *= down;
+#pragma unroll
+            for (int q = 0; q < N; ++q) o[q] *= down;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const bool on = j0 + j < n;
+                const float f = on ? ex2(ml[j].x - base) : 0.0f;
+                l = fmaf(on ? ml[j].y : 0.0f, f, l);
+#pragma unroll
+                for (int q = 0; q < N; ++q) o[q] = fmaf(on ? v[j][q] : 0.0f, f, o[q]);
+            }
+        }
+        const float inv = 1.0f / l;
+        uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)head * HD + lane * N);
+#pragma unroll
+        for (int q = 0; q < N; q += 2) to[q / 2] = pack2<T>(o[q] * inv, o[q + 1] * inv);
+    }
+    if (!waited) pdl_wait();
+}
+
+// Joins the pieces of R query rows next to one another in their tiles -- those of x, then those of y -- and stores them. AHEAD pieces of each are on their way at a time.
+template <typename T, int HD, int R, int AHEAD>
+__device__ __forceinline__ void join_rows(const Cuts &x, const Cuts &y, uint16_t *const (&to)[R])
+{
+    constexpr int N = HD / 32;                               // numbers of a lane, next to one another
+    const int lane = threadIdx.x & 31, n = x.count + y.count;
+    float top[R], l[R], o[R][N];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        top[r] = -INFINITY; l[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[r][k] = 0.0f;
+    }
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += AHEAD) {
+        float2 ml[R][AHEAD];
+        float v[R][AHEAD][N];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {                    // behind the last one it again, with no weight
+            const int k = min(j0 + j, n - 1);
+            const long long at = k < x.count ? (long long)k * x.step : (long long)(k - x.count) * y.step;
+            const float *from = (k < x.count ? x.acc : y.acc) + at * HD + lane * N;
+            const float2 *tops = (k < x.count ? x.top : y.top) + at;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                ml[r][j] = tops[r];
+                if constexpr (N >= 4) {
+#pragma unroll
+                    for (int q = 0; q < N; q += 4) *reinterpret_cast<float4 *>(&v[r][j][q]) = *reinterpret_cast<const float4 *>(from + r * HD + q);
+                } else *reinterpret_cast<float2 *>(v[r][j]) = *reinterpret_cast<const float2 *>(from + r * HD);
+            }
+        }
+        asm volatile("" ::: "memory");                      // all of them before the first is used
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float higher = top[r];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) higher = fmaxf(higher, ml[r][j].x);
+            const float base = higher == -INFINITY ? 0.0f : higher, down = ex2(top[r] - base);
+            top[r] = higher;
+            l[r] *= down;
+#pragma unroll
+            for (int q = 0; q < N; ++q) o[r][q] *= down;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const bool on = j0 + j < n;
+                const float f = on ? ex2(ml[r][j].x - base) : 0.0f;
+                l[r] = fmaf(on ? ml[r][j].y : 0.0f, f, l[r]);
+#pragma unroll
+                for (int q = 0; q < N; ++q) o[r][q] = fmaf(on ? v[r][j][q] : 0.0f, f, o[r][q]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float inv = 1.0f / l[r];
+        uint32_t *out = reinterpret_cast<uint32_t *>(to[r] + lane * N);
+#pragma unroll
+        for (int q = 0; q < N; q += 2) out[q / 2] = pack2<T>(o[r][q] * inv, o[r][q + 1] * inv);
+    }
+}
+
+// The same where there are more query rows than warps: a key / value head's query rows of all requests are one sequence, of which a warp takes up to JOIN_CHUNK in a
+// row, looks up their places together and joins two at a time. Four portions, 38 000 rows of two or three pieces: 31 us, and 51 one by one; 96 rows of 35
+// pieces, hd 256: 12 one by one, and 21 so.
+template <typename T, int HD>
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+attn_join_rows_kernel(const __grid_constant__ b200_paged_attn_args a, const __grid_constant__ Shape shape, const Pieces few, const Pieces many)
+{
+    extern __shared__ __align__(1024) char smem[];
+    __shared__ Plan p;
+    const int warp = threadIdx.x >> 5;
+    // The lengths are older than the kernel before this one, which started after all that came before it had ended: only its pieces are waited for.
+    if (!make_plan(a, shape, smem, p)) { pdl_wait(); return; }
+    pdl_launch_dependents();
+    bool waited = false;
+    const int G = shape.by_g.d, per_head = p.row[p.n_req] * G, workers = gridDim.x * JOIN_WARPS;
+    const int chunk = (int)min(((long long)per_head * a.n_kv + workers - 1) / workers, (long long)JOIN_CHUNK), chunks = chunk ? (per_head + chunk - 1) / chunk : 0;      // of a head
+    for (long long c = blockIdx.x * JOIN_WARPS + warp; c < (long long)chunks * a.n_kv; c += workers) {
+        const int h = (int)(c / chunks), begin = ((int)(c % chunks)) * chunk, end = min(begin + chunk, per_head);
+        int r = 0, past = 0, group = -1, shift = 0, y_from = 0, y_past = 0, x_from = 0, x_past = 0;     // request, end of its rows; where the cuts looked up hold
         Cuts x = {}, y = {};
-#pragma unroll 1
-        for (int head = first; head < first + heads; ++head) {
-            const int i = (row - p.row[r]) * G + head - h * G, j = group >= 0 ? i + (p.small[r] - p.small[p.group[group]]) * G : 0;
-            if (head == first || !(i % FEW_ROWS) || !(j % FEW_ROWS)) {       // another tile, it may be
-                y = way_of(p, own) ? cuts_of<1>(p, own, many, p.n_groups + r, h, i, HD) : cuts_of<0>(p, own, few, p.n_groups + r, h, i, HD);
-                if (group >= 0) x = way_of(p, shared) ? cuts_of<1>(p, shared, many, group, h, j, HD) : cuts_of<0>(p, shared, few, group, h, j, HD);
-                x.acc += lane * N; y.acc += lane * N;
-            } else {
-                x.acc += HD; ++x.top; y.acc += HD; ++y.top;
+        for (int at = begin; at < end;) {
+            if (at >= past) {                                // another request
+                r = last_at(p.row, p.n_req, over(at, shape.by_g));
+                past = p.row[r + 1] * G;
+                group = group_of(p, r);
+                if (set_at(p, p.n_groups + r).before > 0) group = -1;    // one set
+                shift = group >= 0 ? (p.small[r] - p.small[p.group[group]]) * G : 0;
+                y_past = x_past = -1;
+                x = {};
             }
-            if (group < 0 && !y.several) continue;           // stored where it was formed
+            const int i = at - p.row[r] * G, j = i + shift;
+            if (i >= y_past) {
+                const Set own = set_at(p, p.n_groups + r);
+                const int way = way_of(p, own), rows = way ? MANY_ROWS : FEW_ROWS;
+                y = way ? cuts_of<1>(p, own, many, p.n_groups + r, h, i, HD) : cuts_of<0>(p, own, few, p.n_groups + r, h, i, HD);
+                y_from = i; y_past = (i / rows + 1) * rows;
+            }
+            if (group >= 0 && j >= x_past) {
+                const Set shared = set_at(p, group);
+                const int way = way_of(p, shared), rows = way ? MANY_ROWS : FEW_ROWS;
+                x = way ? cuts_of<1>(p, shared, many, group, h, j, HD) : cuts_of<0>(p, shared, few, group, h, j, HD);
+                x_from = j; x_past = (j / rows + 1) * rows;
+            }
+            int left = min(min(end, past) - at, y_past - i); // rows that are found at the same places
+            if (group >= 0) left = min(left, x_past - j);
+            if (group < 0 && !y.several) { at += left; continue; }       // stored where they were formed
             if (!waited) { pdl_wait(); waited = true; }
-            const int n = x.count + y.count;
-            auto top_of = [&](int j) { return j < x.count ? x.top + (long long)j * x.step : y.top + (long long)(j - x.count) * y.step; };
-            auto acc_of = [&](int j) { return j < x.count ? x.acc + (long long)j * x.step * HD : y.acc + (long long)(j - x.count) * y.step * HD; };
-            float top = -INFINITY, l = 0.0f, o[N];
-#pragma unroll
-            for (int k = 0; k < N; ++k) o[k] = 0.0f;
-#pragma unroll 1
-            for (int j0 = 0; j0 < n; j0 += AHEAD) {
-                float2 ml[AHEAD];
-                float v[AHEAD][N];
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {            // behind the last one it again, with no weight
-                    const int k = min(j0 + j, n - 1);
-                    const float *from = acc_of(k);
-                    ml[j] = *top_of(k);
-                    if constexpr (N >= 4) {
-#pragma unroll
-                        for (int q = 0; q < N; q += 4) *reinterpret_cast<float4 *>(&v[j][q]) = *reinterpret_cast<const float4 *>(from + q);
-                    } else *reinterpret_cast<float2 *>(v[j]) = *reinterpret_cast<const float2 *>(from);
-                }
-                float higher = top;
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) higher = fmaxf(higher, ml[j].x);
-                const float base = higher == -INFINITY ? 0.0f : higher, down = ex2(top - base);
-                top = higher;
-                l *= down;
-#pragma unroll
-                for (int q = 0; q < N; ++q) o[q] *= down;
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const bool on = j0 + j < n;
-                    const float f = on ? ex2(ml[j].x - base) : 0.0f;
-                    l = fmaf(on ? ml[j].y : 0.0f, f, l);
-#pragma unroll
-                    for (int q = 0; q < N; ++q) o[q] = fmaf(on ? v[j][q] : 0.0f, f, o[q]);
-                }
+            auto out = [&](int k) {
+                const int row = over(at + k, shape.by_g);
+                return static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)(h * G + at + k - row * G) * HD;
+            };
+            const Cuts xs = {x.acc + (long long)(j - x_from) * HD, x.top + (j - x_from), x.count, x.step, true};
+            const Cuts ys = {y.acc + (long long)(i - y_from) * HD, y.top + (i - y_from), y.count, y.step, true};
+            if (left >= 2) {
+                uint16_t *const to[2] = {out(0), out(1)};
+                join_rows<T, HD, 2, (HD > 128 ? 2 : 4)>(xs, ys, to);
+                at += 2;
+            } else {
+                uint16_t *const to[1] = {out(0)};
+                join_rows<T, HD, 1, 8>(xs, ys, to);
+                ++at;
             }
-            const float inv = 1.0f / l;
-            uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.d_out) + (long long)row * a.out_ld + (size_t)head * HD + lane * N);
-#pragma unroll
-            for (int q = 0; q < N; q += 2) to[q / 2] = pack2<T>(o[q] * inv, o[q + 1] * inv);
         }
     }
     if (!waited) pdl_wait();
@@ -233,9 +357,10 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
         if (!pool_map(&map_k, a.d_k_pool, a, box) || !pool_map(&map_v, a.d_v_pool, a, box)) return B200_E_STATE;
     }
     const size_t smem = room.plan_off + plan + 1024;
-    static std::atomic<unsigned long long> pages_done, join_done;
+    static std::atomic<unsigned long long> pages_done, join_done, join_rows_done;
     cudaError_t e = allow_all(attn_pages_kernel<T, HD>, pages_done);
     if (e == cudaSuccess) e = allow_all(attn_join_kernel<T, HD>, join_done);
+    if (e == cudaSuccess) e = allow_all(attn_join_rows_kernel<T, HD>, join_rows_done);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     const int sets = a.n_req + a.n_groups;
@@ -254,7 +379,8 @@ int launch(const b200_paged_attn_args &a, cudaStream_t st)
     ++g_b200_launches;
     L.shape.each = (sets + JOIN_WARPS * 32 - 1) / (JOIN_WARPS * 32);
     const long long blocks = ((long long)a.max_rows * a.n_q + JOIN_WARPS - 1) / JOIN_WARPS, most = (long long)JOIN_BLOCKS * L.shape.blocks;
-    e = launch_chained(attn_join_kernel<T, HD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(JOIN_WARPS * 32), plan, st, a, L.shape, few, many);
+    e = launch_chained(blocks > most ? attn_join_rows_kernel<T, HD> : attn_join_kernel<T, HD>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(JOIN_WARPS * 32), plan, st, a,
+                       L.shape, few, many);
     if (e != cudaSuccess) return (int)e;
     ++g_b200_launches;
     return (int)cudaGetLastError();
