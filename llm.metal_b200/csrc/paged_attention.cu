@@ -321,7 +321,7 @@ Layout layout_of(const b200_paged_attn_args &a)
     L.shape.blocks = sm_count(); 
     const int rings = (int)((ROOM - plan_bytes(a.n_req, a.n_groups)) / few_ring(a.hd));       // hundreds of requests leave less than all of the warps a ring
     L.shape.few_warps = rings < most_few_warps(a.hd) ? rings : most_few_warps(a.hd);
-    L.shape.ratio = a.hd == 64 ? 16.0f : 10.0f;              // from the ends of both kinds of blocks, 64 requests of one prefix of 65521 tokens: together within a tenth
+    L.shape.ratio = a.hd == 64 ? 16 : 10;              // from the ends of both kinds of blocks, 64 requests of one prefix of 65521 tokens: together within a tenth
     L.shape.row_step[0] = (int)((FEW_ROWS * 256 + G - 1) / G); L.shape.row_step[1] = (int)((MANY_ROWS * 256 + G - 1) / G);
     L.shape.each = 1;
     // tiles: all rows in full ones, and one that is not full for each set that has rows; a piece more for each worker

@@ -35,7 +35,7 @@ struct Shape {
     Div by_g, by_kv;
     int few_most, big, blocks, few_warps, each;
     int row_step[2];
-    float ratio;
+    int ratio;
 };
 
 // Where a way's pieces lie in d_work: [slot][rows of a tile][hd] sums and [slot][rows of a tile] (largest score, sum), scores in units of log 2. A tile's piece of
@@ -153,12 +153,14 @@ template <int WAY> __device__ __forceinline__ int stretch(int units, int workers
 }
 
 // Reads the lengths and lays the lines; false (for the whole block) if something does not fit. `mem` holds plan_bytes; for blocks of up to 16 warps.
+// Two kernels lay the same plan with unlike numbers of threads, and the second looks for the pieces where the first has left them: so all sums are of whole numbers, whose
+// order does not matter. (tests/test_cpu_paged_plan.py compares them.)
 // This runs at the head of every launch, from cold instruction caches: short code counts, so loops stay loops. 3.5 thousand clocks for 33 sets (as a function of its
 // own, which reads the launch's arguments from memory, 8).
 __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const Shape &shape, char *mem, Plan &plan)
 {
     __shared__ int4 red[16];
-    __shared__ float2 red_f[16];
+    __shared__ longlong2 red_w[16];
     const int sets = a.n_req + a.n_groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int *const unit = reinterpret_cast<int *>(mem), *const row = unit + 4 * (sets + 1), *const group = row + 3 * a.n_req + 2;
     if (threadIdx.x == 0) {
@@ -211,29 +213,25 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
     // the two lines: (units, tiles) of each, for the sets of this thread, of the warp, of the block
     const int e0 = min(sets, (int)threadIdx.x * shape.each), e1 = min(sets, e0 + shape.each);
     int4 mine = make_int4(0, 0, 0, 0);
-    float size = 0.0f, many_cost = 0.0f;
+    long long size = 0, many_cost = 0;                       // many_cost: in twentieths of a unit of the first way
 #pragma unroll 1
     for (int e = e0; e < e1; ++e) {
         const Set s = set_at(plan, e);
         int n = 0, k = 0;
         const int way = way_of(plan, s);
         if (s.nr > 0 && s.keys > 0) {
-            float cost, most;                                // most: of a head, in floating point: lines of 2^31 units are refused below
             if (way) {
                 k = tiles_of<1>(s);
                 n = line_before<1>(plan, s, k);
                 // a tile whose rows fit into one stream costs two thirds
                 const int last = s.nr - (k - 1) * Cut<1>::ROWS;
-                most = (float)k * (float)(Cut<1>::GAP + 1 + units_of<1>(plan, s, k - 1));
-                cost = (float)n * shape.ratio * (last > Cut<1>::ROWS / 2 ? 1.0f : 1.0f - __fdividef(0.35f, (float)k));
+                size += (long long)k * (Cut<1>::GAP + 1 + units_of<1>(plan, s, k - 1)) * shape.by_kv.d;          // at most: lines of 2^31 units are refused below
+                many_cost += (20LL * n - (last > Cut<1>::ROWS / 2 ? 0 : 7 * (n / k))) * (shape.ratio * shape.by_kv.d);
             } else {
                 k = tiles_of<0>(s);
                 n = line_before<0>(plan, s, k);
-                cost = (float)n;
-                most = (float)k * (float)(Cut<0>::GAP + 1 + units_of<0>(plan, s, k - 1));
+                size += (long long)k * (Cut<0>::GAP + 1 + units_of<0>(plan, s, k - 1)) * shape.by_kv.d;
             }
-            size += most * (float)shape.by_kv.d;
-            if (way) many_cost += cost * (float)shape.by_kv.d;
             n *= shape.by_kv.d; k *= shape.by_kv.d;
         }
         int *const at = unit + e + way * 2 * (sets + 1);     // summed up below, by the same thread
@@ -247,22 +245,22 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, in.x, o), y = __shfl_up_sync(0xffffffffu, in.y, o);
         const int z = __shfl_up_sync(0xffffffffu, in.z, o), w = __shfl_up_sync(0xffffffffu, in.w, o);
-        const float f = __shfl_up_sync(0xffffffffu, size, o), g = __shfl_up_sync(0xffffffffu, many_cost, o);
+        const long long f = __shfl_up_sync(0xffffffffu, size, o), g = __shfl_up_sync(0xffffffffu, many_cost, o);
         if (lane >= o) { in.x += x; in.y += y; in.z += z; in.w += w; size += f; many_cost += g; }
     }
-    if (lane == 31) { red[warp] = in; red_f[warp] = make_float2(size, many_cost); }
+    if (lane == 31) { red[warp] = in; red_w[warp] = make_longlong2(size, many_cost); }
     __syncthreads();
     int4 all = make_int4(0, 0, 0, 0);
     in.x -= mine.x; in.y -= mine.y; in.z -= mine.z; in.w -= mine.w;
-    size = many_cost = 0.0f;
+    size = many_cost = 0;
 #pragma unroll 1
     for (int w = 0; w * 32 * shape.each < sets; ++w) {       // (the others have none)
         const int4 x = red[w];
         if (w < warp) { in.x += x.x; in.y += x.y; in.z += x.z; in.w += x.w; }
         all.x += x.x; all.y += x.y; all.z += x.z; all.w += x.w;
-        size += red_f[w].x; many_cost += red_f[w].y;
+        size += red_w[w].x; many_cost += red_w[w].y;
     }
-    if (size > 2.0e9f) {                                     // lines of 2^31 units: tens of terabytes of keys
+    if (size > 2000000000) {                                 // lines of 2^31 units: tens of terabytes of keys
         if (blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
         return false;
     }
@@ -278,8 +276,10 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
         // blocks for each way: by their shares of the work, no more than have units to begin with, one at least
         int many = 0;
         if (all.z > 0) {
-            const float a1 = many_cost, a0 = (float)all.x;
-            many = all.x == 0 ? shape.blocks : max(1, min(shape.blocks - 1, (int)((float)shape.blocks * __fdividef(a1, a0 + a1) + 0.5f)));
+            const unsigned long long both = 20ULL * all.x + many_cost;
+            const int down = max(0, 42 - __clzll(both));     // 22 bits of each are enough
+            const unsigned part = (unsigned)((unsigned long long)many_cost >> down), whole = (unsigned)(both >> down);
+            many = all.x == 0 ? shape.blocks : max(1, min(shape.blocks - 1, (int)((shape.blocks * part + whole / 2) / whole)));
             many = min(many, (all.z + Cut<1>::LEAST - 1) / Cut<1>::LEAST);
         }
         plan.many_blocks = many;
