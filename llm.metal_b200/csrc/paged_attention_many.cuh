@@ -179,7 +179,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
     __shared__ uint64_t full_bar[MOST_SLOTS], empty_bar[MOST_SLOTS], q_bar[2], s_bar[2][2], p_bar[2][2], o_bar[2][2], alone_bar[2], both_bar, both_done;
     __shared__ uint32_t tmem_sh;
     __shared__ int abort_sh;
-    __shared__ uint32_t special_sh[4][2];
+    __shared__ uint32_t special_sh[6][2];                    // marks of values that are not finite: two of each stream's own, two of both's
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &abort_sh;
     const uint32_t q_tiles = smem_u32(base), ring = q_tiles + 2 * Q_TILE;
@@ -192,7 +192,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
             for (int k = 0; k < 2; ++k) { mbar_init(&p_bar[s][k], 128); mbar_init(&o_bar[s][k], 1); }
         }
         mbar_init(&both_bar, 256); mbar_init(&both_done, 2);
-        for (int i = 0; i < 8; ++i) special_sh[i >> 1][i & 1] = 0;
+        for (int i = 0; i < 12; ++i) special_sh[i >> 1][i & 1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -320,7 +320,9 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     };
                     const int there = u.seen - key0;         // a thread to a key
                     const bool looks = !both || s == 0;
-                    uint32_t *found = special_sh[both ? 2 + both_phase : s];
+                    // By turns (a unit meets once or three times): a warp may write the next unit's marks while another has yet to read these, and who writes those of the
+                    // unit after that has met everyone in between.
+                    uint32_t *found = special_sh[both ? 4 + both_phase : 2 * s + alone_phase];
                     if (looks) {
                         bool special = false;
                         if (r < there && r < MANY_KEYS && u.own) {
