@@ -144,8 +144,8 @@ struct Streams {
     int units[2], n, lead, ahead;        // lead: `ahead`, or all that there are
     __device__ __forceinline__ uint32_t values(int j) const { return lead + j + min(j, n - lead); }
 };
-// (Four units ahead where every other one is a stream's, if the ring has 7 places: the values of a unit whose scores are there then lie in a place whose
-// occupant before them has arrived, so that the parity of its barrier says which of the two is meant.)
+// (Four units ahead where every other one is a stream's, if the ring has 7 places: what lay before the values of a unit whose scores are there was asked for before
+// its keys then, which is_there relies on.)
 __device__ __forceinline__ Streams streams_of(const Plan &p, const Piece &q, int slots)
 {
     Streams w;
@@ -203,6 +203,12 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
     __syncthreads();
     after_sync();
     const uint32_t tmem = tmem_sh;
+    // Whether what passes as the phase-th through a place of the ring has arrived. Where each stream reads every other unit, the other stream's keys or values may have been there before
+    // and may still be on their way, as copies do not land in order; the parity of the barrier of arrivals is then that of the phase before it, which is over. That
+    // the place was given back first decides: it was asked for before something that this stream has seen arrive, and is not given back again without this stream.
+    auto is_there = [&](int slot, uint32_t phase, bool halves) {
+        return __all_sync(0xffffffffu, (!halves || wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag)) && wait_or_abort(&full_bar[slot], phase, abort_flag)) != 0;
+    };
     auto give_up = [&]() { if (!*abort_flag) { *abort_flag = 1; if (a.d_status) atomicOr(a.d_status, B200_PAGED_TIMED_OUT); } };
 
     // Registers: 168 a thread at the launch, 384 threads; 72 for four warps and 216 for the eight with a row of scores a thread are as many.
@@ -312,7 +318,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     // Not all rows see all of these keys: zero weights must not meet infinities or NaN. Values behind the last seen key are made zero; of those
                     // that some rows see, the ones that are not finite are added row by row and then made zero too.
                     const uint32_t v_item = item + w.values(unit), v_at = ring + (v_item % slots) * SLOT;
-                    if (!__all_sync(0xffffffffu, wait_or_abort(&full_bar[v_item % slots], (v_item / slots) & 1, abort_flag))) { ok = false; break; }
+                    if (!is_there(v_item % slots, (v_item / slots) & 1, w.halves)) { ok = false; break; }
                     const bool both = !w.halves && unit < w.units[0];
                     auto meet = [&]() {                      // of all threads that read this unit
                         if (both) { mbar_arrive(&both_bar); ok = __all_sync(0xffffffffu, wait_or_abort(&both_bar, both_phase, abort_flag)); both_phase ^= 1; }
@@ -486,7 +492,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                 after_sync();
                 // A place is free again when both streams have said so, a stream that has no use for it too; the only reader of one says it twice.
                 auto scores = [&](int place, const Place &k) {
-                    if (!ok || !(ok = arrived(&full_bar[k.slot], k.phase))) return;
+                    if (!ok || !(ok = is_there(k.slot, k.phase, halves))) return;
                     after_sync();
                     const uint64_t kd = k_desc + k.slot * (SLOT >> 4);
                     if (one_lane()) {
@@ -501,7 +507,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     __syncwarp();
                 };
                 auto sums = [&](int place, const Place &v) {
-                    if (!ok || !(ok = arrived(&full_bar[v.slot], v.phase) && arrived(&p_bar[s][place], (p_phase >> place) & 1))) return;
+                    if (!ok || !(ok = is_there(v.slot, v.phase, halves) && arrived(&p_bar[s][place], (p_phase >> place) & 1))) return;
                     p_phase ^= 1u << place;
                     after_sync();
                     const uint64_t vd = v_desc + v.slot * (SLOT >> 4);

@@ -76,9 +76,9 @@ class Piece:
         return at
 
 
-def run(pieces, slots, rng, buffers=2, in_order=True):
+def run(pieces, slots, rng, buffers=2, freed_first=True):
     full, empty = [Barrier() for _ in range(slots)], [Barrier(2) for _ in range(slots)]
-    holds, flying = [None] * slots, []                           # the item that lies in a place; copies on their way
+    holds, flying = [None] * slots, {}                           # the item that lies in a place; copies on their way and how long they take: some are late
     queues = [[], []]                                            # what the tensor core has been given by each issuing warp
     queries, done, both = [Barrier(4), Barrier(4)], Barrier(2), Barrier(8)
     scores, sums = ([[Barrier(), Barrier()] for _ in range(2)] for _ in range(2))
@@ -95,14 +95,16 @@ def run(pieces, slots, rng, buffers=2, in_order=True):
             yield
             assert not any(kind == "read" and at % slots == slot for q in queues for kind, at, _ in q), "written while it is read"
             holds[slot] = None
-            flying.append(item)
+            flying[item] = int(10 ** rng.uniform(0, 2.5))
 
     def landing():
         while True:
-            if flying:
-                item = flying.pop(0 if in_order else rng.randrange(len(flying)))
-                holds[item % slots] = item
-                full[item % slots].arrive()
+            for item in list(flying):
+                flying[item] -= 1
+                if not flying[item]:
+                    del flying[item]
+                    holds[item % slots] = item
+                    full[item % slots].arrive()
             yield
 
     def tensor(s):
@@ -126,6 +128,8 @@ def run(pieces, slots, rng, buffers=2, in_order=True):
                 slot = item % slots
                 if p.halves and unit & 1 != s:
                     continue
+                if p.halves and freed_first:
+                    yield from empty[slot].wait(item // slots - 1)
                 yield from full[slot].wait(item // slots)
                 if not p.halves and unit >= mine:
                     empty[slot].arrive()
@@ -160,6 +164,8 @@ def run(pieces, slots, rng, buffers=2, in_order=True):
                     yield from settled(j)
                 if p.hidden[unit]:
                     item = starts[turn] + p.values(unit)
+                    if p.halves and freed_first:
+                        yield from empty[item % slots].wait(item // slots - 1)
                     yield from full[item % slots].wait(item // slots)
                     assert holds[item % slots] == item, "values of another unit"
                     together = not p.halves and unit < p.units[0]
@@ -210,7 +216,7 @@ def run(pieces, slots, rng, buffers=2, in_order=True):
                 except StopIteration:
                     del live[name]
                     left -= 1
-        state = [(b.phase, b.count) for b in every], len(flying), [len(q) for q in queues], left
+        state = [(b.phase, b.count) for b in every], sum(flying.values()), [len(q) for q in queues], left
         idle, last = (idle + 1, last) if state == last else (0, state)
         assert idle < 500, f"{sorted(map(str, live))} wait for ever"
 
@@ -226,9 +232,22 @@ def test_everyone_reads_what_was_written_for_the_unit(slots):
     runs(120, slots, slots)
 
 
+@pytest.mark.parametrize("slots", [6, 8, 9])
+def test_waiting_for_the_own_copy_alone_is_not_enough(slots):
+    """Where the other stream's keys have yet to land in the place before, its barrier has the parity of an earlier phase's end."""
+    with pytest.raises(AssertionError, match="one phase taken for another|another unit"):
+        runs(3000, slots, 2, freed_first=False)
+
+
 def test_one_buffer_of_marks_is_not_enough():
     with pytest.raises(AssertionError, match="marks of another unit"):
         runs(400, 9, 1, buffers=1)
+
+
+def test_the_kernel_waits_for_the_place_first():
+    s = source()
+    assert "(!halves || wait_or_abort(&empty_bar[slot], phase ^ 1, abort_flag)) && wait_or_abort(&full_bar[slot], phase, abort_flag)" in s
+    assert s.count("is_there(") == 3 and s.count("&full_bar[") == 5      # by rows, for scores and for sums; besides: set up, filled twice, passed on
 
 
 def test_the_kernel_has_two_buffers_of_marks():
