@@ -84,8 +84,8 @@ int b200_pages_release(const b200_pages_args *a, void *stream);
  *   k, v   rounded to the pool's type, stored at slot d_slot[m]; a slot outside the pool is left out
  *   q      rounded likewise, stored to row m of d_q: what b200_paged_attn reads
  * With use_pdl the weights (d_q_gamma, d_k_gamma, d_inv_freq) are read ahead of the wait for the kernel before.
- * *d_rows rows (a device word, at most max_rows): the last of b200_pages_extend's d_row_start. Two rows of one slot: one
- * of them is kept.
+ * *d_rows rows (a device word): the last of b200_pages_extend's d_row_start. If it is negative or more than max_rows, nothing
+ * is stored and *d_status says so. Two rows of one slot: one of them is kept.
  * ---------------------------------------------------------------------- */
 typedef struct b200_paged_store_args {
     int wtype, n_q, n_kv, hd, page, n_pages, max_rows;

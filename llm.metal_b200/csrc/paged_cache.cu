@@ -244,6 +244,10 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __g
     };
     int h0 = blockIdx.y * heads_per_block + warp * HEADS + lane / LANES;
     load(h0);
+    if (rows < 0 || rows > a.max_rows) {
+        if (m == 0 && blockIdx.y == 0 && threadIdx.x == 0) report(a.d_status, B200_PAGED_BAD_LENGTH);
+        return;
+    }
     if (m >= rows) return;
     if (threadIdx.x < HALF && a.d_inv_freq) {
         constexpr double TURN = 6.283185307179586476925, PER_TURN = 0.15915494309189533577;
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __g
         s_cos[threadIdx.x] = cs; s_sin[threadIdx.x] = sn;
     }
     const bool in_pool = slot >= 0 && slot < a.n_pages * a.page;
-    if (!in_pool && threadIdx.x == 0 && blockIdx.y == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_PAGE);
+    if (!in_pool && threadIdx.x == 0 && blockIdx.y == 0) report(a.d_status, B200_PAGED_BAD_PAGE);
     __syncthreads();
     float cs[N], sn[N];
     *reinterpret_cast<float4 *>(cs) = *reinterpret_cast<const float4 *>(s_cos + d);

@@ -213,6 +213,20 @@ def test_store_leaves_out_slots_outside_the_pool(pkg):
     assert (d["v"] == 5).all()
 
 
+@pytest.mark.parametrize("count", [-1, 7, 2 ** 31 - 1, -2 ** 31])
+def test_store_of_a_count_that_does_not_fit(pkg, count):
+    page, n_pages, max_rows = 16, 10, 6
+    d, _, _, _ = stored(pkg, "f16", 4, 2, 64, page, max_rows, max_rows, [5] * 6, [1, 2, 3, 20, 50, 159], n_pages)
+    for name, fill in (("q", 7.0), ("k", 3.0), ("v", 5.0)):
+        d[name].fill_(fill)
+    d["count"].fill_(count)
+    a = args(pkg.PagedStoreArgs, wtype=1, n_q=4, n_kv=2, hd=64, page=page, n_pages=n_pages, max_rows=max_rows, eps=1e-6, d_qkv=d["qkv"], qkv_ld=d["qkv"].shape[1], d_rows=d["count"],
+             d_slot=d["slot"], d_pos=d["pos"], d_k_pool=d["k"], d_v_pool=d["v"], d_q=d["q"], q_ld=d["q"].shape[1], d_status=d["status"])
+    assert pkg.lib().b200_paged_store(C.byref(a), None) == 0
+    assert d["status"].tolist() == [2]
+    assert (d["q"] == 7).all() and (d["k"] == 3).all() and (d["v"] == 5).all()
+
+
 def test_store_behind_four_billion_elements(pkg):
     page, n_pages = 16, 2 ** 32 // (16 * 2 * 128) + 9                  # element offsets past 32 bits
     slots = [page * n_pages - 1, page * (n_pages - 8) + 3, 0]
