@@ -58,7 +58,8 @@ extern "C" {
  *
  * b200_pages_release: requests with d_new[r] != 0 give their pages back, request after request, to the top of the stack
  * (d_free has room for n_pages), and d_len_out[r] becomes 0, d_len[r] for the others. The table keeps its
- * numbers. d_base, d_row_start, d_slot, d_pos and max_rows are not used. All or nothing, likewise.
+ * numbers. d_base, d_row_start, d_slot, d_pos and max_rows are not used. All or nothing, likewise. A page number outside the
+ * pool goes onto the stack as the table has it, so that the stack's height stays that of the lengths, with B200_PAGED_BAD_PAGE.
  *
  * d_len_out may be d_len and d_free_n_out may be d_free_n; no other two arrays may overlap.
  * ---------------------------------------------------------------------- */

@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
     // aligned for them.
     const int thread = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x, shift = 31 - __clz(a.page);
     const int pages_each = total.y > threads ? 4 : 1, rows_each = total.x > threads ? 4 : 1;
+    unsigned outside = 0;
 #pragma unroll 1
     for (int p = pages_each * thread; p < total.y; p += pages_each * threads) {
         int q = owner_of(s_page, n, p);
@@ -117,12 +118,14 @@ __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b20
         for (int k = 0; k < 4; ++k) {
             if (k >= pages_each || p + k >= total.y) break;
             while (q + 1 < n && s_page[q + 1] <= p + k) ++q;
-            if (RELEASE) a.d_free[free_n + p + k] = a.d_table[(size_t)q * a.table_ld + (p + k - s_page[q])];
-            else a.d_table[(size_t)q * a.table_ld + ((s_len[q] + a.page - 1) >> shift) + (p + k - s_page[q])] = a.d_free[free_n - 1 - p - k];
+            if (RELEASE) {
+                const int id = a.d_table[(size_t)q * a.table_ld + (p + k - s_page[q])];
+                a.d_free[free_n + p + k] = id;
+                if (id < 0 || id >= a.n_pages) outside = B200_PAGED_BAD_PAGE;
+            } else a.d_table[(size_t)q * a.table_ld + ((s_len[q] + a.page - 1) >> shift) + (p + k - s_page[q])] = a.d_free[free_n - 1 - p - k];
         }
     }
-    if (RELEASE) return;
-    unsigned outside = 0;
+    if (RELEASE) { report(a.d_status, outside); return; }
     const bool wide = ((reinterpret_cast<uintptr_t>(a.d_slot) | reinterpret_cast<uintptr_t>(a.d_pos)) & 15) == 0;
 #pragma unroll 1
     for (int m = rows_each * thread; m < total.x; m += rows_each * threads) {

@@ -138,6 +138,21 @@ def test_pages_outside_the_pool_give_no_slot(pkg):
     assert slot[:12] == [-1] * 12 and all(0 <= s < 160 for s in slot[12:15])
 
 
+@pytest.mark.parametrize("table_ld", [6, 600])                     # one block, and a cluster of them
+@pytest.mark.parametrize("page_id", [-1, 10, 2 ** 31 - 1, -2 ** 31])
+def test_release_reports_pages_outside_the_pool(pkg, page_id, table_ld):
+    t = Tables(pkg, 4, 16, table_ld, 10, 64, seed=4)
+    t.extend([5, 20, 3, 1])
+    t.d["table"][0, 0] = page_id
+    t.release([0, 1, 0, 1])                                          # not among them
+    assert t.d["status"].tolist() == [0]
+    t.lists[0][0] = page_id
+    t.release([1, 0, 1, 0])
+    assert t.d["status"].tolist() == [4]
+    t.d["status"].zero_()
+    t.check()                                                        # on the stack as it stood, and the rest in its place
+
+
 # ------------------------------------------------------------------ the writer
 
 def stored(pkg, dtype, n_q, n_kv, hd, page, rows, max_rows, pos, slots, n_pages, gamma=True, rotate=True, pad=0, seed=0):
