@@ -74,18 +74,15 @@ typedef CUresult (*encode_fn_t)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// (Asked for once: a second thread that calls meanwhile waits for the answer.)
 inline encode_fn_t encode_fn()
 {
-    static encode_fn_t fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    static const encode_fn_t fn = [] {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<encode_fn_t>(p);
-    }
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<encode_fn_t>(p) : nullptr;
+    }();
     return fn;
 }
 
