@@ -109,7 +109,9 @@ int b200_paged_store(const b200_paged_store_args *a, void *stream);
  * none) of the pages d_prefix_table[g][prefix_ld]. Requests outside every group have no prefix; n_groups 0: no
  * request has. The pages of a prefix are read once for every 256 query rows (rows times n_q / n_kv) of its group, up to hd 128, and
  * for every 16 above; a request that brings 128 of them by itself, a portion of a prompt, reads its prefix for itself.
- * Tokens that a row does not see have no influence on it, whatever their slots hold (infinities and NaN too).
+ * Tokens that a row does not see have no influence on it, whatever their slots hold (infinities and NaN too). Scores, largest scores and
+ * sums are fp32; each weight is rounded to the pool's type before it meets its value (half a step; in binary16 2^-32 of the row's
+ * largest weight at least), and the result once more. (b200_rows_attn has two planes of queries, and weights and results of fp32.)
  *
  * If a length or a range does not fit its buffer, the call leaves all of its output as it was and *d_status says
  * so. A page number outside the pool is not read; what the rows that would see it come out as is undefined.

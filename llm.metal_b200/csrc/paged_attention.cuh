@@ -31,6 +31,9 @@ template <typename T> __device__ __forceinline__ float to_float(uint16_t b)
     if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(b));
     else return __uint_as_float((uint32_t)b << 16);
 }
+// Weights are powers of two over the largest score so far, less this: binary16 ends at 2^15.99 above and has its full precision down to 2^-14 only, so that of weights of 1 at most half
+// its range would lie idle, and 65 536 keys of 2^-26 each, 2^-10 of the sum together, would vanish from the weighted one. `most`: such that the largest weight is 2^15. bfloat16 has fp32's range.
+template <typename T> __device__ __forceinline__ constexpr float weight_lift(int most) { return std::is_same<T, __half>::value ? (float)most : 0.0f; }
 // Whether one of the eight elements of a 16-byte word is infinite or NaN.
 template <typename T> __device__ __forceinline__ bool any_special(const uint4 &v)
 {

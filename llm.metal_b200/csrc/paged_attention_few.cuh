@@ -3,7 +3,8 @@
 // pass with a running maximum. What bounds it is memory: 16 rows take 64 operations a byte of cache at most, and the eight warps of an SM hold enough bytes in
 // flight: 64 requests of 1500 tokens, 8 key / value heads of 128, 4 query heads to each, 82 us, 4.8 TB/s with the head of the launch and the join (floor 60). Warps
 // share nothing, so that there is no barrier in the loop. Scores, maxima, sums and results are fp32; weights are rounded to the
-// cache's type for the second product, by at most half a step each, which is what the results' own rounding is.
+// cache's type for the second product, as its two operands have one type: by half a step each, which is what the results' own rounding is, down to 2^-29 of the largest weight in
+// binary16 and by 2^-40 of it at most below that (weight_lift).
 #pragma once
 #include "paged_attention.cuh"
 
@@ -43,7 +44,7 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
     constexpr int HALF_STAGE = FEW_KEYS * HD * 2, STAGE = 2 * HALF_STAGE;
     const int lane = threadIdx.x & 31, g = lane >> 2, cq = lane & 3;
     const uint16_t *kp = static_cast<const uint16_t *>(a.d_k_pool), *vp = static_cast<const uint16_t *>(a.d_v_pool);
-    const float c = a.scale * 1.4426950408889634f;
+    const float c = a.scale * 1.4426950408889634f, lift = weight_lift<T>(15);
     const int page_shift = 31 - __clz(a.page);
     const Div by_g = p.shape.by_g;
 
@@ -120,7 +121,7 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
                 mma16<T>(sc[0], q[ks], b[0], b[1]);
                 mma16<T>(sc[1], q[ks], b[2], b[3]);
             }
-            float top[2] = {m[0], m[1]};
+            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
@@ -134,6 +135,7 @@ __device__ void few_worker(const b200_paged_attn_args &a, const Plan &p, const P
             for (int r = 0; r < 2; ++r) {
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                top[r] = fmaxf(m[r], top[r] - lift);
                 base[r] = top[r] == -INFINITY ? 0.0f : top[r];
             }
             if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {

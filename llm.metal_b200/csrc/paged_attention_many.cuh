@@ -5,8 +5,8 @@
 // rows on the same keys, or, where a tile has 128 rows at most, the same rows on every other unit of 64 keys, each stream with a maximum, sum and result of its own.
 // Per unit and stream: S = Q K^T (128 x 64, one of two places in tensor memory, so that the next scores are there when these are done with), the weights
 // P = 2^(c S - m) back into S's place as 16-bit pairs, O += P V with P as the operand from tensor memory and V as it lies, [key][hd] (the product's
-// second operand along its rows). m is the largest score so far only as far as it must be: O is rescaled when it is exceeded by a factor of 2^8, which both 16-bit
-// types have room for.
+// second operand along its rows). m is the largest score so far, less 7 in binary16 (weight_lift), and that only as far as it must be: O is rescaled when the largest weight would
+// be more than 2^8 times that, 2^15. Weights are rounded by half a step down to 2^-21 of the largest one in binary16 and by 2^-32 of it at most below that.
 //   warp 0      pages into a ring of shared memory: TMA, a box of 64 numbers by up to 64 tokens a lane, keys and values by turns
 //   warps 1, 2  the products of stream 0, of stream 1: one lane issues them
 //   warps 4-7   stream 0: queries into shared memory, softmax, results; warps 8-11 stream 1. A thread to a row.
@@ -220,6 +220,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
         // the sign goes into the queries; a scale of zero weighs all seen keys alike, and hidden ones, at minus infinity, not at all
         const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.17549435e-38f);
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        constexpr float LIFT = weight_lift<T>(7);
         uint32_t turn = 0, item = 0, s_phase = 0, even = 0, odd = 0, alone_phase = 0, both_phase = 0;      // even, odd: products with weights of the first and of the second place, before this piece
         bool ok = true;
         Walk<1> walk(p, blockIdx.x);
@@ -287,7 +288,7 @@ __device__ __forceinline__ void many_block(const CUtensorMap &map_k, const CUten
                     float big4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int q = 0; q < 64; ++q) big4[q & 3] = fmaxf(big4[q & 3], __uint_as_float(x[q]));
-                    const float big = valid ? fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3])) * c : -INFINITY;   // (what lies in other rows must not decide)
+                    const float big = valid ? fmaxf(fmaxf(big4[0], big4[1]), fmaxf(big4[2], big4[3])) * c - LIFT : -INFINITY;   // (what lies in other rows must not decide)
                     if (__any_sync(0xffffffffu, big > top + 8.0f)) {     // (true too for the first)
                         const float higher = fmaxf(top, big), f = top == -INFINITY ? 0.0f : ex2(top - higher);
                         if (__any_sync(0xffffffffu, top != -INFINITY)) {

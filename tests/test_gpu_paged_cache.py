@@ -347,6 +347,32 @@ def test_scores_of_all_sizes(pkg):
         s.check()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,new,n_req", [(64, 1, 148), (128, 1, 148), (256, 1, 74), (64, 40, 18), (128, 40, 18), (128, 200, 18)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_one_strong_key_before_many_weak_ones(pkg, dtype, hd, new, n_req, shared):
+    """8192 keys of 2^-26 of the first one's weight each make up all of the result, in tiles that few workers cut. Its error: the results' rounding and the weights' -- half a step of
+    the type each, in binary16 at least half of its smallest number, 2^-25, where the largest weight is 2^15 (2^7 where there are many rows): 2^-40 (2^-32) of the largest each --,
+    sums of n terms (n 2^-23), and the score, 18, by 2^-22 of it."""
+    n, kv, value = 8192, 8, 8.0
+    own = new if shared else n
+    s = Step(pkg, dtype, kv, kv, hd, 128, [own] * n_req, [new] * n_req, range(n_req + 1) if shared else (), [n] * n_req if shared else (), scale=1.0)
+    s.k.zero_(); s.v.fill_(value); s.q.zero_()
+    strong, at = 16.0, (s.p_table if shared else s.table)[:, 0].long()
+    s.k[at, :, 0, 0], s.v[at, :, 0] = strong, 0
+    s.q.view(s.max_rows, kv, hd)[:, :, 0] = 26 * math.log(2) / strong
+    s.run()
+    assert s.status.tolist() == [0]
+    score, eps = strong * s.q[0, 0].double().item(), torch.finfo(s.type).eps
+    weak = (n if shared else n - new) + torch.arange(new, device="cuda").double()[:, None]     # keys that row i sees, without the strong one
+    share = weak * math.exp(-score)
+    want = value * share / (1 + share)
+    tiny = (2.0 ** -40 if new == 1 else 2.0 ** -32) if dtype == "f16" else 0.0
+    bound = want * (eps * 1.01 + 2 * score * 2.0 ** -22 + 2 * n * 2.0 ** -23) + tiny * weak * value
+    off = (s.out[:s.rows].double().view(n_req, new, kv * hd) - want).abs() / bound
+    assert off.max() <= 1, off.max().item()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.05, 0.7])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_scales(pkg, scale, hd):
