@@ -114,7 +114,8 @@ int b200_paged_store(const b200_paged_store_args *a, void *stream);
  * largest weight at least), and the result once more. (b200_rows_attn has two planes of queries, and weights and results of fp32.)
  *
  * If a length or a range does not fit its buffer, the call leaves all of its output as it was and *d_status says
- * so. A page number outside the pool is not read; what the rows that would see it come out as is undefined.
+ * so. So it does for work of 2^31 units (16 query rows by 16 keys, from 33 query rows of a request or group on and up to hd 128 256 by 64, and up to 13
+ * more for each 16 or 256 rows): a prompt of 185 000 tokens as one portion, at 32 query heads of 256. A page number outside the pool is not read; what the rows that would see it come out as is undefined.
  * d_work: b200_paged_attn_work_bytes(a) bytes, 16-byte aligned, for this call alone while it runs; nothing is kept in it
  * from one call to the next. Calls that may run at the same time need a d_work each.
  * ---------------------------------------------------------------------- */

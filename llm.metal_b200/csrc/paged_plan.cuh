@@ -138,12 +138,12 @@ template <int WAY> __device__ __forceinline__ int units_of(const Plan &p, const 
 }
 // Where the t-th tile of a head begins on the line, its gap included. A request's tiles see about row_step / 256 keys more from one to the next: their places come
 // from the sum of that progression, with one unit more a tile for what rounding takes, and a tile's gap is what its units leave (GAP - 2 at least).
-template <int WAY> __device__ __forceinline__ int line_before(const Plan &p, const Set &s, int t)
+template <int WAY, typename Place = int> __device__ __forceinline__ Place line_before(const Plan &p, const Set &s, int t)
 {
     constexpr int GAP = Cut<WAY>::GAP, KEYS = Cut<WAY>::KEYS;
-    if (!s.own) return t * (GAP + units_of<WAY>(p, s, 0));
+    if (!s.own) return (Place)t * (GAP + units_of<WAY>(p, s, 0));
     const long long keys = (long long)(s.keys - s.rows) * t + (((long long)p.shape.row_step[WAY] * t * (t + 1)) >> 9);
-    return t * (GAP + 1 + units_before_own<WAY>(s)) + (int)(keys / KEYS);
+    return (Place)t * (GAP + 1 + units_before_own<WAY>(s)) + (Place)(keys / KEYS);
 }
 
 // Units of a worker: equal stretches, and none so short that joining costs more than it spreads.
@@ -218,20 +218,22 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
     for (int e = e0; e < e1; ++e) {
         const Set s = set_at(plan, e);
         int n = 0, k = 0;
+        long long line = 0;                                  // of a head
         const int way = way_of(plan, s);
         if (s.nr > 0 && s.keys > 0) {
             if (way) {
                 k = tiles_of<1>(s);
-                n = line_before<1>(plan, s, k);
+                line = line_before<1, long long>(plan, s, k);
                 // a tile whose rows fit into one stream costs two thirds
                 const int last = s.nr - (k - 1) * Cut<1>::ROWS;
-                size += (long long)k * (Cut<1>::GAP + 1 + units_of<1>(plan, s, k - 1)) * shape.by_kv.d;          // at most: lines of 2^31 units are refused below
+                n = (int)line;
                 many_cost += (20LL * n - (last > Cut<1>::ROWS / 2 ? 0 : 7 * (n / k))) * (shape.ratio * shape.by_kv.d);
             } else {
                 k = tiles_of<0>(s);
-                n = line_before<0>(plan, s, k);
-                size += (long long)k * (Cut<0>::GAP + 1 + units_of<0>(plan, s, k - 1)) * shape.by_kv.d;
+                line = line_before<0, long long>(plan, s, k);
+                n = (int)line;
             }
+            size += line * shape.by_kv.d;
             n *= shape.by_kv.d; k *= shape.by_kv.d;
         }
         int *const at = unit + e + way * 2 * (sets + 1);     // summed up below, by the same thread
@@ -260,7 +262,7 @@ __device__ __forceinline__ bool make_plan(const b200_paged_attn_args &a, const S
         all.x += x.x; all.y += x.y; all.z += x.z; all.w += x.w;
         size += red_w[w].x; many_cost += red_w[w].y;
     }
-    if (size > 2000000000) {                                 // lines of 2^31 units: tens of terabytes of keys
+    if (size > INT_MAX) {                                    // places on the lines are 32-bit numbers
         if (blockIdx.x == 0 && threadIdx.x == 0 && a.d_status) atomicOr(a.d_status, B200_PAGED_BAD_LENGTH);
         return false;
     }

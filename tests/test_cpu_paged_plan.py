@@ -27,7 +27,7 @@ def laid(pkg, tmp_path_factory):
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wno-unknown-pragmas", "-shared", "-fPIC", str(at / "plan_on_host.cpp"), "-o", str(at / "plan.so")], check=True)
     lib = C.CDLL(str(at / "plan.so"))
 
-    def plan(threads, new, total, starts=(), prefix=(), n_q=8, n_kv=1, page=16, ratio=16, few_warps=8):
+    def plan(threads, new, total, starts=(), prefix=(), n_q=8, n_kv=1, page=16, ratio=16, few_warps=8, few_most=FEW_MOST, big=BIG):
         n, m = len(new), len(prefix)
         ints = lambda x: (C.c_int * max(1, len(x)))(*x)           # noqa: E731
         rows = [0]
@@ -40,7 +40,7 @@ def laid(pkg, tmp_path_factory):
             setattr(a, field, C.addressof(x))
         a.d_status = C.addressof(status)
         out = (C.c_int * (5 + 4 * (n + m + 1) + n + 1))()
-        fine = lib.plan_on_host(C.byref(a), FEW_MOST, BIG, BLOCKS, few_warps, ratio, threads, out)
+        fine = lib.plan_on_host(C.byref(a), few_most, big, BLOCKS, few_warps, ratio, threads, out)
         assert status.value == (0 if fine else pkg.B200_PAGED_BAD_LENGTH)
         return list(out) if fine else None
 
@@ -88,3 +88,18 @@ def test_both_kernels_divide_the_blocks_alike(laid, n, seed):
         for first in range(a - 40 * 16, a + 40 * 16, 16):
             if first > 0:
                 both(first)
+
+
+@pytest.mark.parametrize("rows,n_q,n_kv,wide,fits", [(131072, 32, 8, False, True), (180000, 32, 8, False, True), (190000, 32, 8, False, False), (1 << 20, 8, 1, True, True),
+                                                     (1 << 20, 56, 8, True, True), (1 << 20, 128, 8, True, False), (1 << 20, 1024, 1, True, False), (1 << 20, 1024, 1024, False, False)])
+def test_lines_are_refused_from_two_to_the_31_units_on(laid, rows, n_q, n_kv, wide, fits):
+    """A prompt as one portion: tiles of 256 rows by units of 64 keys, or, above head dimension 128, of 16 by 16, of which a row's tile sees half on average."""
+    tile, unit, gap = (256, 64, 8) if wide else (16, 16, 2)
+    tiles = -(-rows * (n_q // n_kv) // tile)
+    units = n_kv * sum(gap + 1 + (min((t + 1) * tile // (n_q // n_kv), rows)) / unit for t in range(0, tiles, 64)) * 64      # (every 64th tile stands for its neighbours)
+    assert abs(units / 2 ** 31 - 1) > 0.01 and (units < 2 ** 31) == fits
+    for threads in (384, 128):
+        plan = laid(threads, [rows], [rows], n_q=n_q, n_kv=n_kv, **({} if wide else dict(few_most=2 ** 31 - 1, big=2 ** 31 - 1, few_warps=4)))
+        assert (plan is not None) == fits
+        if fits:
+            assert abs(plan[4 if wide else 3] / units - 1) < 0.01
