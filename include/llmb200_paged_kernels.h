@@ -121,7 +121,7 @@ int b200_paged_store(const b200_paged_store_args *a, void *stream);
  * ---------------------------------------------------------------------- */
 typedef struct b200_paged_attn_args {
     int wtype, n_q, n_kv, hd, page, n_pages, max_rows;
-    float scale;                                             /* finite */
+    float scale;                                             /* finite, times log2(e) too: below 2.3e38 */
     const void *d_q; long long q_ld;                         /* rows q_ld elements apart, a multiple of 8; 16-byte aligned */
     const void *d_k_pool, *d_v_pool;
     void *d_out; long long out_ld;                           /* likewise; n_q * hd elements of the pool's type a row */

@@ -398,7 +398,7 @@ extern "C" int b200_paged_attn(const b200_paged_attn_args *ap, void *stream)
     if (!ap) return B200_E_BADARG;
     const b200_paged_attn_args &a = *ap;
     if (const int rc = check_sizes(a)) return rc;
-    if (!std::isfinite(a.scale)) return B200_E_BADARG;
+    if (!std::isfinite(a.scale * 1.4426950408889634f)) return B200_E_BADARG;        // (weights are powers of two)
     if (a.max_rows == 0 || a.n_req == 0) return 0;
     if (!a.d_q || !a.d_k_pool || !a.d_v_pool || !a.d_out || !a.d_row_start || !a.d_len || !a.d_table || !a.d_work) return B200_E_BADARG;
     if (a.n_groups && (!a.d_group_start || !a.d_prefix_len || (a.prefix_ld && !a.d_prefix_table))) return B200_E_BADARG;

@@ -81,6 +81,11 @@ def test_attention_refusals(pkg, lib, more, code):
     assert lib.b200_paged_attn(None, None) == BADARG
 
 
+@pytest.mark.parametrize("scale", [2.4e38, -2.4e38, 3.4e38])
+def test_scales_that_overflow_as_powers_of_two(pkg, lib, scale):
+    assert lib.b200_paged_attn(C.byref(attn(pkg, scale=scale)), None) == BADARG
+
+
 def test_nothing_to_do_is_no_error(pkg, lib):
     assert lib.b200_paged_store(C.byref(store(pkg, max_rows=0)), None) == 0
     assert lib.b200_paged_attn(C.byref(attn(pkg, max_rows=0)), None) == 0
