@@ -86,7 +86,7 @@ int b200_pages_release(const b200_pages_args *a, void *stream);
  *   q      rounded likewise, stored to row m of d_q: what b200_paged_attn reads
  * With use_pdl the weights (d_q_gamma, d_k_gamma, d_inv_freq) are read ahead of the wait for the kernel before.
  * *d_rows rows (a device word): the last of b200_pages_extend's d_row_start. If it is negative or more than max_rows, nothing
- * is stored and *d_status says so. Two rows of one slot: one of them is kept.
+ * is stored and *d_status says so. b200_pages_extend gives no slot twice; of two rows of one slot each element is one of the two's.
  * ---------------------------------------------------------------------- */
 typedef struct b200_paged_store_args {
     int wtype, n_q, n_kv, hd, page, n_pages, max_rows;

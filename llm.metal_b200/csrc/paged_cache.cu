@@ -58,7 +58,10 @@ __device__ __forceinline__ void report(unsigned *status, unsigned bits)
 }
 
 constexpr int TABLE_BLOCKS = 8;          // a portable cluster
-constexpr int TABLE_ROWS = 2048;         // below this many rows (pages for release) one block does it
+// Up to this many rows (pages for release) one block does it, which a launch starts sooner. Us in a captured run, one block and the cluster, extend: 32 requests and 32 rows 2.6 and 3.3, 2048
+// rows 4.1 and 4.2, 3000 rows 4.3 and 4.3, 4096 rows 4.5 and 4.3, 8192 rows 6.3 and 4.1; 1024 requests and 2048 rows 4.4 and 4.6, 3000 rows 4.8 and 4.6; release: 1024 requests and 2048
+// pages 3.8 and 4.1, 4096 pages 4.4 and 4.1.
+constexpr int TABLE_ROWS = 2048;
 
 template <bool RELEASE>
 __global__ void __launch_bounds__(1024) pages_kernel(const __grid_constant__ b200_pages_args a)
@@ -209,6 +212,10 @@ template <typename T> __device__ __forceinline__ uint16_t to_bits(float x)
 }
 
 constexpr int STORE_WARPS = 8, STORE_AHEAD = 2;
+// Up to STORE_FEW rows a block has one round of heads, or 32 rows would run on 32 SMs; above, all heads of a row, which forms the angles once. Us in a captured run, one round and all heads:
+// 32 / 8 heads of 128, 32 rows 2.1 and 3.0, 128 rows 2.9 and 3.3, 256 rows 4.2 and 3.8, 512 rows 6.2 and 4.8; 16 / 8 heads of 128, 32 rows 2.3 and 2.5, 128 rows 2.6 and
+// 2.7, 256 rows 3.2 and 3.0, 512 rows 4.7 and 3.8; 16 / 2 heads of 64 and 4 / 1 of 256 are one round or little more, and the same either way.
+constexpr int STORE_FEW = 192;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __grid_constant__ b200_paged_store_args a, int heads_per_block)
@@ -315,8 +322,7 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) paged_store_kernel(const __g
 template <typename T>
 int launch_store(const b200_paged_store_args &a, cudaStream_t st)
 {
-    // few rows: one round of heads to a block, or 32 rows would run on 32 SMs; many: all heads of a row in one block, which forms the angles once
-    const int heads = a.n_q + 2 * a.n_kv, per = a.max_rows <= 512 ? STORE_WARPS * 256 / a.hd : heads;
+    const int heads = a.n_q + 2 * a.n_kv, per = a.max_rows <= STORE_FEW ? STORE_WARPS * 256 / a.hd : heads;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.max_rows, (heads + per - 1) / per);
     cfg.blockDim = dim3(STORE_WARPS * 32);

@@ -242,6 +242,17 @@ def test_store_of_a_count_that_does_not_fit(pkg, count):
     assert (d["q"] == 7).all() and (d["k"] == 3).all() and (d["v"] == 5).all()
 
 
+@pytest.mark.parametrize("rows", [2, 40, 700])
+def test_store_of_one_slot_for_all_rows(pkg, rows):
+    """Every element is that of one of them, and nothing else is written."""
+    page, n_pages = 16, 3
+    d, _, k, v = stored(pkg, "bf16", 4, 2, 64, page, rows, rows, [9] * rows, [21] * rows, n_pages, rotate=False, gamma=False)
+    for pool, fill, x in ((d["k"], 3.0, k), (d["v"], 5.0, v)):
+        assert (pool[1, :, 5][None] == x.bfloat16()).any(0).all()
+        pool[1, :, 5] = fill
+        assert (pool == fill).all()
+
+
 def test_store_behind_four_billion_elements(pkg):
     page, n_pages = 16, 2 ** 32 // (16 * 2 * 128) + 9                  # element offsets past 32 bits
     slots = [page * n_pages - 1, page * (n_pages - 8) + 3, 0]
