@@ -401,6 +401,16 @@ def test_pages_of_all_sizes_hold_shared_prefixes(pkg, page, hd):
         s.check()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(16, 2, 64), (32, 8, 128), (4, 1, 256)])
+@pytest.mark.parametrize("total,new", [([700, 90, 3], [1, 1, 1]), ([700, 0, 300], [1, 0, 140]), ([5, 5, 5], [0, 0, 0])])
+def test_attention_of_few_rows_under_a_large_bound(pkg, dtype, n_q, n_kv, hd, total, new):
+    s = Step(pkg, dtype, n_q, n_kv, hd, 16, total, new, [0, 3], [1000], max_rows=8192)
+    s.run()
+    s.check()
+    assert s.status.tolist() == [0]
+
+
 @pytest.mark.parametrize("q_pad,out_pad", [(8, 16), (136, 0)])
 def test_attention_strides(pkg, q_pad, out_pad):
     s = Step(pkg, "bf16", 16, 8, 128, 16, [50, 300, 9], [1, 5, 9], [0, 3], [70], q_pad=q_pad, out_pad=out_pad, table_pad=5)
