@@ -1,7 +1,7 @@
 // Attention of a step's new rows over pages (sm_100a): each row over its request's own tokens, and over a prefix that its group shares. One launch works on all keys
 // (paged_plan.cuh: how they are cut; paged_attention_few.cuh and paged_attention_many.cuh: the two ways), one block to an SM, and a second one joins the pieces
 // of tiles that were cut. (Two launches for the two ways, one after the other, and plans and joins without care for cold instruction caches: 77 us for 32
-// answers to a prompt of 8199 tokens that take 40 now, 28 for four short chats that take 14; floors 16 and 0.5.)
+// answers to a prompt of 8199 tokens that take 42 now, 28 for four short chats that take 14; floors 16 and 0.5.)
 #include "paged_attention_few.cuh"
 #include "paged_attention_many.cuh"
 

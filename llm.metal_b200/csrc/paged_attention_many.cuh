@@ -12,7 +12,7 @@
 //   warps 4-7   stream 0: queries into shared memory, softmax, results; warps 8-11 stream 1. A thread to a row.
 // What bounds it: for tiles of 128 rows memory, once the copies are under way; for full ones the chain weights -> product -> next scores. A unit of 64 keys by 256 rows
 // takes 1.9 thousand clocks (hd 128), of which the tensor core is busy most (scores of 64 columns seem to cost it as much as 128 would) and the rows' warps 1.6, 1.0 of them exponentials; four
-// portions of 125 .. 811 tokens behind 4096, 32 / 8 heads, 181 us: 830 TFLOP/s, 0.51 of the measured product. On the way there, the same launch: units of
+// portions of 125 .. 811 tokens behind 4096, 32 / 8 heads, 179 us: 840 TFLOP/s, 0.52 of the measured product. On the way there, the same launch: units of
 // 128 keys, whose next scores wait for the products of these, 224 us; units of 64 issued by one lane that divides and makes addresses for each step 314,
 // by a whole warp in uniform registers 210, by one for each stream 185. A quarter of the weights by a polynomial, and scores read from tensor memory a unit early, gave nothing.
 // Every wait is bounded; on a timeout the block reports it, lets copies in flight land, frees its tensor memory and returns.

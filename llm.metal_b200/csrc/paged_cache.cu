@@ -201,7 +201,7 @@ int launch_pages(const b200_pages_args *ap, void *stream)
 }
 
 // ---- new rows into their slots ------------------------------------------------------------------------------------------------
-// Bound by memory: 4 bytes read and 2 written a number; 8191 rows of 32 heads of 128 take 46 us, 4.4 TB/s, where a copy reaches 6.6. hd / 8 lanes hold a
+// Bound by memory: 4 bytes read and 2 written a number; 8191 rows of 32 heads of 128 take 41 us, 4.9 TB/s, where a copy reaches 6.6. hd / 8 lanes hold a
 // head, each four numbers of its lower half and the four that they turn with, so that the norm is a few shuffles and the rotation stays in
 // the lane. (A warp to a head of 128, four numbers a lane: 140 instructions a head, 50 us.) The angle pos * inv_freq is formed in 64 bits (exact) and brought
 // into one turn before the 32-bit sine and cosine: as a 32-bit product it is off by pos * 2^-24, more than binary16's step from position 8000 on. q, k and v are rounded once, to the type of the cache that the tensor cores read.
